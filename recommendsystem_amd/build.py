@@ -20,7 +20,10 @@ OBJDIR = os.path.join(HERE, "build")
 LIB = os.path.join(LIBDIR, "librs_hip.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950", "-ffp-contract=off",
-         "-Wall", "-Wno-unused-function", "-I", CSRC]
+         "-Wall", "-Wno-unused-function", "-I", CSRC,
+         # no packed fp32 instructions: single fp32 operations everywhere (the host pass does not know the feature and
+         # warns about it; the warning says nothing about the device code)
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # Per-file additions.  interact.hip: MFMA results are consumed by vector instructions right away, so the products are
 # written to ordinary vector registers instead of accumulation registers that have to be copied out first.
 EXTRA_FLAGS = {"interact.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}

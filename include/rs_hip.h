@@ -581,6 +581,37 @@ int rs_shard_pack(const int* plan, const int* route, int F, int cap, int d, cons
 int rs_shard_counts(const long long* recv_idx, int N, int F, const int* capf, const int* boff, int S, int* sub_cnt,
                     const int* plan, const int* route, int cap, int* slot_map, int B, int Fdiv, rs_stream_t stream);
 
+/* ---- sequence operators: layer norm, rotary positions (fp32 / bf16 / fp16) ---------- */
+/* No counterpart in the reference, whose interactions see one sample's fields and no history.  Type codes (dtype): 0 fp32,
+ * 1 bf16, 2 fp16.  Strides are in elements; the last dimension is always contiguous. */
+
+/* s = round(x + r) (r null: s = x, nothing is written to s), y = (s - mean) rstd w + b over the last dimension of
+ * [M, N]: model/utils/Layers.py:30,44 holds nn.LayerNorm behind a Linear (rs_ln_fwd is that form, fp32, with the
+ * activation); this one takes 16-bit types, rows of any stride ldx / ldr and a residual stream, and keeps two floats per
+ * row (mean, rstd; each may be null) for the backward instead of a normalised copy.  w / b (null: 1 / 0) are of type
+ * param_dtype, which is dtype or fp32.  y and s are contiguous.
+ * Backward: dx = rstd (g - avg g - xhat avg(g xhat)) + ds with g = dy w (ds null: none; it is the gradient that reaches s
+ * past the norm), dw = sum_rows dy xhat, db = sum_rows dy (each may be null), in a fixed order of summation.  The
+ * gradient of r is dx.  workspace: rs_layer_norm_bwd_workspace_floats(M, N) floats when dw or db is wanted. */
+int rs_layer_norm_partial_rows(int M, int N);
+size_t rs_layer_norm_bwd_workspace_floats(int M, int N);
+int rs_layer_norm_fwd(int dtype, int param_dtype, const void* x, long long ldx, const void* r, long long ldr, int M, int N,
+                      const void* w, const void* b, float eps, void* y, void* s, float* mean, float* rstd,
+                      rs_stream_t stream);
+int rs_layer_norm_bwd(int dtype, int param_dtype, const void* dy, long long lddy, const void* s, long long lds,
+                      const float* mean, const float* rstd, const void* w, const void* ds, long long ldds, int M, int N,
+                      void* dx, void* dw, void* db, float* workspace, size_t workspace_floats, rs_stream_t stream);
+
+/* Turns the first R (even) of the D elements of every head of q [B, T, Hq, D] and k [B, T, Hk, D] by the angles of the
+ * tokens' positions and copies the rest; outputs contiguous.  Pair i is elements (i, i + R/2), or (2i, 2i + 1) with
+ * `interleaved`; cos_table / sin_table [max_positions, R/2].  positions: int64 (positions_i64) or int32, strides pb / pt
+ * over samples / tokens (pb = 0: shared).  A position outside the table reads row 0 and sets *err_flag.  inverse: by the
+ * negative angle, the way gradients go.  Hq or Hk may be 0.  Outputs must not overlap inputs. */
+int rs_rotary(int dtype, const void* q, long long qb, long long qt, long long qh, int Hq, const void* k, long long kb,
+              long long kt, long long kh, int Hk, int B, int T, int D, int R, int interleaved, const void* positions,
+              int positions_i64, long long pb, long long pt, const float* cos_table, const float* sin_table,
+              int max_positions, int inverse, void* q_out, void* k_out, int* err_flag, rs_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

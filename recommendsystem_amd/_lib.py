@@ -132,6 +132,14 @@ _SIGS = {
     "rs_dropout_apply": [c_f32p, c_f32p, L, F, C.c_ulonglong, C.c_uint, C.c_ulonglong, c_i64p, c_stream],
     "rs_axpy_f32": [F, c_f32p, c_f32p, L, c_stream],
     "rs_loss_add_reg": [c_f32p, c_f32p, c_i32p, c_f32p, I, c_stream],
+    # layer_norm.hip
+    "rs_layer_norm_fwd": [I, I, C.c_void_p, L, C.c_void_p, L, I, I, C.c_void_p, C.c_void_p, F, C.c_void_p, C.c_void_p, c_f32p,
+                          c_f32p, c_stream],
+    "rs_layer_norm_bwd": [I, I, C.c_void_p, L, C.c_void_p, L, c_f32p, c_f32p, C.c_void_p, C.c_void_p, L, I, I, C.c_void_p,
+                          C.c_void_p, C.c_void_p, c_f32p, SZ, c_stream],
+    # rotary.hip
+    "rs_rotary": [I, C.c_void_p, L, L, L, I, C.c_void_p, L, L, L, I, I, I, I, I, I, C.c_void_p, I, L, L, c_f32p, c_f32p, I, I,
+                  C.c_void_p, C.c_void_p, c_i32p, c_stream],
     # shard.hip
     "rs_shard_route": [c_i32p, I, I, c_i64p, I, c_i32p, c_i32p, I, c_i64p, c_i32p, c_i32p, c_stream],
     "rs_shard_gather": [c_i64p, c_i64p, c_i64p, I, I, c_i32p, c_i32p, I, I, I, c_f32p, c_f32p, c_f32p, c_f32p, I, I,
@@ -195,6 +203,8 @@ _PLAIN = {
     "rs_sparse_touched_dot_groups": (I, [I, I]),
     "rs_act_bwd_num_partials": (I, [L]),
     "rs_interact_partial_rows": (I, [I]),
+    "rs_layer_norm_partial_rows": (I, [I, I]),
+    "rs_layer_norm_bwd_workspace_floats": (SZ, [I, I]),
     "rs_ffm_bwd_num_partials": (I, [I, I]),
     "rs_sparse_bwd_wide_num_partials": (I, [I, I]),
 }

@@ -1,0 +1,49 @@
+// Element types of the sequence operators: fp32, bf16 and fp16 in memory, fp32 in registers.
+#pragma once
+#include "common.h"
+
+enum { RS_F32 = 0, RS_BF16 = 1, RS_F16 = 2 };
+
+typedef float rs_f32x4 __attribute__((ext_vector_type(4)));
+typedef float rs_f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 rs_bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 rs_f16x8 __attribute__((ext_vector_type(8)));
+
+// V = the 16-byte vector of T, E = its elements.
+template <typename T> struct RsVec;
+template <> struct RsVec<float> { typedef rs_f32x4 V; static constexpr int E = 4; };
+template <> struct RsVec<__bf16> { typedef rs_bf16x8 V; static constexpr int E = 8; };
+template <> struct RsVec<_Float16> { typedef rs_f16x8 V; static constexpr int E = 8; };
+
+// VE consecutive elements as fp32: one 16-byte access (VE = RsVec<T>::E, p aligned to 16 bytes) or a single one.
+// Stores round to nearest even once.
+template <typename T, int VE> __device__ __forceinline__ void rs_load(const T* p, float* v) {
+    if constexpr (VE == 1) {
+        v[0] = (float)*p;
+    } else {
+        const typename RsVec<T>::V x = *(const typename RsVec<T>::V*)p;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) v[e] = (float)x[e];
+    }
+}
+template <typename T, int VE> __device__ __forceinline__ void rs_store(T* p, const float* v) {
+    if constexpr (VE == 1) {
+        *p = (T)v[0];
+    } else {
+        typename RsVec<T>::V x;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) x[e] = (T)v[e];
+        *(typename RsVec<T>::V*)p = x;
+    }
+}
+
+// Any number of workgroups (a grid dimension holds 2^32 lanes): kernels launched so take rs_block_id() for their number
+// and leave when it is past the last one.
+static inline dim3 rs_grid(long long blocks) {
+    const long long x = blocks < (1 << 22) ? blocks : (1 << 22);
+    return dim3((unsigned)x, (unsigned)((blocks + x - 1) / x));
+}
+__device__ __forceinline__ long long rs_block_id() { return (long long)blockIdx.y * gridDim.x + blockIdx.x; }
+
+static inline int rs_elem_bytes(int dtype) { return dtype == RS_F32 ? 4 : 2; }
+static inline bool rs_aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }

@@ -8,6 +8,7 @@ from __future__ import annotations
 from typing import List, Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import ops
 from .ops import ACT_CODES, FieldLayout, SparsePlan
@@ -882,3 +883,63 @@ class _BiInteractionFn(torch.autograd.Function):
 
 def bi_interaction(emb):
     return _BiInteractionFn.apply(emb)
+
+
+# -------------------------------------------------------------------------------------------------
+# sequence operators: layer norm with a residual stream, rotary positions
+# -------------------------------------------------------------------------------------------------
+class _LayerNormFn(torch.autograd.Function):
+    """y = norm(x) or (y, s) = (norm(s), s) with s = x + residual."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, eps):
+        ctx.set_materialize_grads(False)
+        y, s, mean, rstd = ops.layer_norm_fwd(x, weight, bias, eps, residual)
+        ctx.save_for_backward(s, mean, rstd, weight)
+        ctx.bias = None if bias is None else bias.dtype
+        return y if residual is None else (y, s)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, ds=None):
+        s, mean, rstd, weight = ctx.saved_tensors
+        need_w, need_b = ctx.needs_input_grad[1], ctx.needs_input_grad[2]
+        if dy is None:                       # only the residual stream was used
+            dx = ds
+            dw = torch.zeros_like(weight) if need_w else None
+            db = torch.zeros(s.shape[-1], dtype=ctx.bias, device=s.device) if need_b else None
+        else:
+            dx, dw, db = ops.layer_norm_bwd(dy, s, mean, rstd, weight, ds=ds, want_params=need_w or need_b,
+                                            param_dtype=ctx.bias)
+        return dx, dw if need_w else None, db if need_b else None, dx if ctx.needs_input_grad[3] else None, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
+    """Layer norm over the last dimension (ops.layer_norm_fwd) with its gradients: y, or (y, s) with a residual, s = x +
+    residual being the stream that goes on past the norm."""
+    return _LayerNormFn.apply(x, weight, bias, residual, eps)
+
+
+class _RotaryFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, positions, q, k):
+        ctx.set_materialize_grads(False)
+        ctx.table = table
+        ctx.save_for_backward(positions)
+        return ops.rotary(table, positions, q, k)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq, dk=None):
+        positions, = ctx.saved_tensors
+        if dq is not None and dk is not None:
+            dq, dk = ops.rotary(ctx.table, positions, dq, dk, inverse=True)
+        elif dq is not None or dk is not None:
+            d = ops.rotary(ctx.table, positions, dq if dq is not None else dk, inverse=True)
+            dq, dk = (d, None) if dq is not None else (None, d)
+        return None, None, dq, dk
+
+
+def rotary(table, positions, q, k=None):
+    """Rotary positions (ops.rotary) with their gradients: q's, or (q's, k's)."""
+    return _RotaryFn.apply(table, positions, q, k)

@@ -229,6 +229,23 @@ class Dropout(nn.Dropout):
         return Fn.dropout(x, self.p, self.salt)
 
 
+class LayerNorm(nn.LayerNorm):
+    """nn.LayerNorm over the last dimension (same parameters and state_dict keys) on the HIP kernels, for float32, bfloat16
+    and float16 inputs, with the residual add of a pre-norm block in the same launch: forward(x, residual) returns (y, s)
+    with s = x + residual.  The norms inside MLPBlock / ResidualMLPBlock (Layers.py:39-47,84-94) keep their own kernel,
+    which also applies the activation."""
+
+    def __init__(self, normalized_shape, eps=1e-5, elementwise_affine=True, bias=True):
+        if not isinstance(normalized_shape, int) and len(normalized_shape) != 1:
+            raise RSError(f"LayerNorm: normalises the last dimension only, got {tuple(normalized_shape)}")
+        super().__init__(normalized_shape, eps=eps, elementwise_affine=elementwise_affine, bias=bias)
+
+    def forward(self, x, residual=None):
+        if x.shape[-1:] != self.normalized_shape:
+            raise RSError(f"LayerNorm: last dimension must be {self.normalized_shape[0]}, got {tuple(x.shape)}")
+        return Fn.layer_norm(x, self.weight, self.bias, self.eps, residual)
+
+
 def _activation_module(name: str):
     name = name.lower()
     if name == "relu":

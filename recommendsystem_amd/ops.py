@@ -6,6 +6,7 @@ on torch's current stream.
 """
 from __future__ import annotations
 
+import math
 import os
 from typing import List, Optional
 
@@ -1764,3 +1765,203 @@ def axpy(a: float, x: torch.Tensor, y: torch.Tensor):
     _chk(x, torch.float32, "x")
     _chk(y, torch.float32, "y", x.shape)
     call("rs_axpy_f32", float(a), ptr(x), ptr(y), x.numel(), stream())
+
+
+# ---------------------------------------------------------------------------------------------
+# sequence operators: layer norm with a residual stream, rotary positions (fp32 / bf16 / fp16)
+# ---------------------------------------------------------------------------------------------
+_ELEM_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _elem_code(t: torch.Tensor, name: str) -> int:
+    code = _ELEM_CODES.get(t.dtype)
+    if code is None:
+        raise RSError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
+    return code
+
+
+def _same_device(*named):
+    """All tensors (None allowed) on one GPU; returns it."""
+    dev = None
+    for name, t in named:
+        if t is None:
+            continue
+        require_cuda(t)
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise RSError(f"{name}: is on {t.device}, the first operand on {dev}")
+    return dev
+
+
+def _call_on(dev, name: str, *args):
+    """call() on the current stream of the operands' device, whichever device is current."""
+    if dev.index == torch._C._cuda_getDevice():
+        call(name, *args, stream())
+    else:
+        with torch.cuda.device(dev):
+            call(name, *args, stream())
+
+
+def _norm_rows(t: torch.Tensor, name: str, like: torch.Tensor):
+    """t as [rows, N] with contiguous elements in a row (a copy only where its strides allow no such view), and the row
+    stride."""
+    if t.dtype != like.dtype or t.shape != like.shape:
+        raise RSError(f"{name}: expected {like.dtype} {tuple(like.shape)}, got {t.dtype} {tuple(t.shape)}")
+    N = t.shape[-1]
+    r = t.reshape(-1, N) if t.numel() else t.reshape(0, N)
+    if (N > 1 and r.stride(1) != 1) or (r.shape[0] > 1 and r.stride(0) < N):
+        r = r.contiguous()
+    return r, (r.stride(0) if r.shape[0] > 1 else N)
+
+
+def _norm_param_code(x: torch.Tensor, weight, bias) -> int:
+    """Element code of the weight and the bias (x's type or float32; the same for both)."""
+    N = x.shape[-1]
+    dtype = None
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is None:
+            continue
+        if tuple(p.shape) != (N,) or not p.is_contiguous():
+            raise RSError(f"layer_norm: {name} must be a contiguous vector of {N}, got {tuple(p.shape)}")
+        if p.dtype not in (x.dtype, torch.float32) or (dtype is not None and p.dtype != dtype):
+            raise RSError(f"layer_norm: weight and bias must both be {x.dtype} or both float32, got {name} {p.dtype}")
+        dtype = p.dtype
+    return _ELEM_CODES[dtype if dtype is not None else x.dtype]
+
+
+def layer_norm_fwd(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5,
+                   residual: Optional[torch.Tensor] = None):
+    """s = x + residual (rounded to x's type; s = x without one) and y = (s - mean) * rstd * weight + bias over the last
+    dimension.  x: [..., N], float32 / bfloat16 / float16; weight and bias: [N] of x's type or float32, each may be None.
+    Returns (y, s, mean, rstd): y and s like x, mean and rstd float32 with one value per row for layer_norm_bwd."""
+    code = _elem_code(x, "layer_norm")
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise RSError(f"layer_norm: nothing to normalise in shape {tuple(x.shape)}")
+    pcode = _norm_param_code(x, weight, bias)
+    dev = _same_device(("x", x), ("weight", weight), ("bias", bias), ("residual", residual))
+    N = x.shape[-1]
+    x2, ldx = _norm_rows(x, "x", x)
+    M = x2.shape[0]
+    if M > 0x7FFFFFFF or N > 0x3FFFFFFF:
+        raise RSError(f"layer_norm: {M} rows of {N} are too many")
+    r2, ldr = (None, 0) if residual is None else _norm_rows(residual, "residual", x)
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    s = x if residual is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
+    stats = torch.empty((2, M), dtype=torch.float32, device=dev)
+    mean, rstd = stats[0], stats[1]
+    _call_on(dev, "rs_layer_norm_fwd", code, pcode, ptr(x2), ldx, ptr(r2), ldr, M, N, ptr(weight), ptr(bias), float(eps), ptr(y),
+             None if residual is None else ptr(s), ptr(mean), ptr(rstd))
+    return y, s, mean, rstd
+
+
+def layer_norm_bwd(dy: torch.Tensor, s: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, weight: Optional[torch.Tensor] = None,
+                   ds: Optional[torch.Tensor] = None, want_params: bool = True, param_dtype=None):
+    """Gradients of layer_norm_fwd from dy (of y) and ds (of s past the norm; None: none): (dx, dw, db).  dx, of s's type,
+    is the gradient of x and of the residual alike; dw and db are [N] of the weight's type (param_dtype, default s's type,
+    where there is no weight), None without want_params.  The row sums are added in a fixed order."""
+    code = _elem_code(s, "layer_norm")
+    if s.dim() == 0 or s.shape[-1] == 0:
+        raise RSError(f"layer_norm: nothing to normalise in shape {tuple(s.shape)}")
+    dev = _same_device(("s", s), ("dy", dy), ("mean", mean), ("rstd", rstd), ("weight", weight), ("ds", ds))
+    N = s.shape[-1]
+    s2, lds = _norm_rows(s, "s", s)
+    d2, ldd = _norm_rows(dy, "dy", s)
+    q2, ldq = (None, 0) if ds is None else _norm_rows(ds, "ds", s)
+    M = s2.shape[0]
+    _chk(mean, torch.float32, "mean", (M,))
+    _chk(rstd, torch.float32, "rstd", (M,))
+    pdt = weight.dtype if weight is not None else (param_dtype or s.dtype)
+    if pdt not in (s.dtype, torch.float32):
+        raise RSError(f"layer_norm: parameters must be {s.dtype} or float32, got {pdt}")
+    pcode = _norm_param_code(s, weight, None) if weight is not None else _ELEM_CODES[pdt]
+    dx = torch.empty(s.shape, dtype=s.dtype, device=dev)
+    dw = db = work = None
+    floats = 0
+    if want_params:
+        dw = torch.empty(N, dtype=pdt, device=dev)
+        db = torch.empty(N, dtype=pdt, device=dev)
+        floats = _lib.lib().rs_layer_norm_bwd_workspace_floats(M, N)
+        # per call: two captured graphs, or two streams, never share the partial sums
+        work = torch.empty(max(floats, 1), dtype=torch.float32, device=dev)
+    _call_on(dev, "rs_layer_norm_bwd", code, pcode, ptr(d2), ldd, ptr(s2), lds, ptr(mean), ptr(rstd), ptr(weight), ptr(q2), ldq, M,
+             N, ptr(dx), ptr(dw), ptr(db), ptr(work), floats)
+    return dx, dw, db
+
+
+class RotaryTable:
+    """cos and sin [max_positions, rotary_dim / 2] of position * base^(-2i / rotary_dim), computed in 64 bits and kept in
+    32.  `interleaved`: pair i is the neighbours (2i, 2i + 1) of a head, else the elements (i, i + rotary_dim / 2).
+
+    Long contexts: `factor` > 1 slows the angles down.  Without `original_positions` all of them by that factor; with
+    it, a pair that turns `ramp[1]` times or more over the original length keeps its speed, one that turns `ramp[0]` times
+    or less is slowed by the whole factor, those between by a share that falls linearly with their turns.  `amplitude`
+    multiplies cos and sin."""
+
+    def __init__(self, max_positions: int, rotary_dim: int, device, base: float = 10000.0, interleaved: bool = False,
+                 factor: float = 1.0, original_positions: Optional[int] = None, ramp=(1.0, 32.0), amplitude: float = 1.0):
+        if rotary_dim <= 0 or rotary_dim % 2 or max_positions <= 0 or max_positions > 0x7FFFFFFF:
+            raise RSError(f"RotaryTable: needs an even rotary_dim and positions, got {rotary_dim}, {max_positions}")
+        if not base > 0 or not factor > 0 or (original_positions is not None and not ramp[0] < ramp[1]):
+            raise RSError(f"RotaryTable: base {base}, factor {factor} or ramp {ramp} out of range")
+        device = torch.device(device)
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        self.max_positions, self.rotary_dim, self.interleaved, self.device = int(max_positions), int(rotary_dim), bool(interleaved), device
+        freq = float(base) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
+        if original_positions is None:
+            freq = freq / factor
+        else:
+            turns = original_positions * freq / (2 * math.pi)
+            keep = ((turns - ramp[0]) / (ramp[1] - ramp[0])).clamp(0, 1)
+            freq = freq * (keep + (1 - keep) / factor)
+        angle = torch.arange(max_positions, dtype=torch.float64, device=device)[:, None] * freq.to(device)
+        self.cos = (angle.cos() * amplitude).float()
+        self.sin = (angle.sin() * amplitude).float()
+        self.err_flag = torch.zeros(1, dtype=torch.int32, device=device)
+
+    def check_positions(self):
+        """Raise IndexError if a rotation saw a position outside the table since the last check (device sync; such a
+        position is taken as 0, so nothing faults)."""
+        if int(self.err_flag.item()) != 0:
+            self.err_flag.zero_()
+            raise IndexError(f"rotary: position outside 0..{self.max_positions - 1}")
+
+
+def _heads_view(t: torch.Tensor, name: str, shape=None, dtype=None) -> torch.Tensor:
+    """A [B, T, H, D] operand whose last dimension is contiguous (a copy only where it is not)."""
+    if t.dim() != 4 or (shape is not None and tuple(t.shape) != tuple(shape)):
+        raise RSError(f"{name}: expected [B, T, H, D]{'' if shape is None else ' = ' + str(tuple(shape))}, got {tuple(t.shape)}")
+    if dtype is not None and t.dtype != dtype:
+        raise RSError(f"{name}: expected {dtype}, got {t.dtype}")
+    return t if t.shape[3] <= 1 or t.stride(3) == 1 else t.contiguous()
+
+
+def rotary(table: RotaryTable, positions: torch.Tensor, q: torch.Tensor, k: Optional[torch.Tensor] = None, inverse: bool = False):
+    """q [B, T, Hq, D] (and k [B, T, Hk, D]) with the first table.rotary_dim elements of every head turned by the angles of
+    `positions` ([T] or [B, T], int64 or int32) and the others as they are; one launch, new contiguous tensors.  inverse:
+    by the negative angles, the way gradients go.  Returns q's, or (q's, k's)."""
+    code = _elem_code(q, "rotary")
+    q = _heads_view(q, "q")
+    B, T, Hq, D = q.shape
+    Hk = 0
+    if k is not None:
+        k = _heads_view(k, "k", dtype=q.dtype)
+        Hk = k.shape[2]
+        if k.shape[:2] != q.shape[:2] or k.shape[3] != D:
+            raise RSError(f"rotary: k {tuple(k.shape)} does not go with q {tuple(q.shape)}")
+    if table.rotary_dim > D:
+        raise RSError(f"rotary: the table turns {table.rotary_dim} elements, heads have {D}")
+    if positions.dtype not in (torch.int64, torch.int32) or positions.shape not in ((T,), (B, T)):
+        raise RSError(f"rotary: positions must be int64 or int32 [{T}] or [{B}, {T}], got {positions.dtype} {tuple(positions.shape)}")
+    if (Hq + Hk) * D > 1 << 24 or B * T > 0x7FFFFFFF:
+        raise RSError(f"rotary: {B * T} tokens of {Hq + Hk} heads of {D} are too many")
+    dev = _same_device(("q", q), ("k", k), ("positions", positions), ("table", table.cos))
+    pb, pt = positions.stride() if positions.dim() == 2 else (0, positions.stride(0))
+    qo = torch.empty((B, T, Hq, D), dtype=q.dtype, device=dev)
+    ko = torch.empty((B, T, Hk, D), dtype=q.dtype, device=dev) if k is not None else None
+    qs, ks = q.stride(), (k.stride() if k is not None else (0, 0, 0))
+    _call_on(dev, "rs_rotary", code, ptr(q), qs[0], qs[1], qs[2], Hq, ptr(k), ks[0], ks[1], ks[2], Hk, B, T, D, table.rotary_dim,
+             int(table.interleaved), ptr(positions), int(positions.dtype == torch.int64), pb, pt, ptr(table.cos), ptr(table.sin),
+             table.max_positions, int(inverse), ptr(qo), ptr(ko), ptr(table.err_flag))
+    return qo if k is None else (qo, ko)

@@ -581,7 +581,7 @@ int rs_shard_pack(const int* plan, const int* route, int F, int cap, int d, cons
 int rs_shard_counts(const long long* recv_idx, int N, int F, const int* capf, const int* boff, int S, int* sub_cnt,
                     const int* plan, const int* route, int cap, int* slot_map, int B, int Fdiv, rs_stream_t stream);
 
-/* ---- sequence operators: layer norm, rotary positions (fp32 / bf16 / fp16) ---------- */
+/* ---- sequence operators: layer norm, rotary positions, attention (fp32 / bf16 / fp16) ---------- */
 /* No counterpart in the reference, whose interactions see one sample's fields and no history.  Type codes (dtype): 0 fp32,
  * 1 bf16, 2 fp16.  Strides are in elements; the last dimension is always contiguous. */
 
@@ -611,6 +611,30 @@ int rs_rotary(int dtype, const void* q, long long qb, long long qt, long long qh
               long long kt, long long kh, int Hk, int B, int T, int D, int R, int interleaved, const void* positions,
               int positions_i64, long long pb, long long pt, const float* cos_table, const float* sin_table,
               int max_positions, int inverse, void* q_out, void* k_out, int* err_flag, rs_stream_t stream);
+
+/* Attention: o = softmax(scale q k^T over the visible keys) v for q [B, Tq, Hq, D] and k, v [B, Tk, Hk, D], D <= 128, Hq a
+ * multiple of Hk (query heads h Hq/Hk .. share key head h); b / t / h strides of every operand in elements.  Row i of
+ * sample b sees key j where j < lengths[b] and i < query_lengths[b] (device int32 [B], null: all; clamped to 0..T) and,
+ * with causal != 0, j <= i + start, start = query_starts[b] (device int32 [B]) or query_start where that is null.  A row
+ * that sees nothing: o = 0, lse = -inf, zero gradients.  Keys, values and rows behind the lengths may hold anything.
+ * o [B, Tq, Hq, D] contiguous; lse [B, Hq, Tq] fp32 (null: not wanted), natural logarithm of the sum of exponentials.
+ * workspace (16-byte aligned): rs_attention_fwd_workspace_floats(..) floats, 0 for most shapes: few rows over many keys
+ * are split over the keys and joined by a second launch.
+ * Backward: dq, dk, dv contiguous, of the operands' type, every element written; lse as the forward left it; workspace
+ * rs_attention_bwd_workspace_floats(..) floats.  No atomics: results do not change from run to run.
+ * Stands beside rs_afm_fwd / _bwd (model/AFM/AFM.py:36-56), which pools field pairs with one softmax per sample. */
+size_t rs_attention_fwd_workspace_floats(int dtype, int B, int Tq, int Tk, int Hq, int Hk, int D);
+size_t rs_attention_bwd_workspace_floats(int B, int Tq, int Hq);
+int rs_attention_fwd(int dtype, const void* q, long long qb, long long qt, long long qh, const void* k, long long kb, long long kt,
+                     long long kh, const void* v, long long vb, long long vt, long long vh, int B, int Tq, int Tk, int Hq, int Hk,
+                     int D, const int* lengths, const int* query_lengths, int causal, const int* query_starts, int query_start,
+                     float scale, void* o, float* lse, float* workspace, size_t workspace_floats, rs_stream_t stream);
+int rs_attention_bwd(int dtype, const void* go, long long gb, long long gt, long long gh, const void* q, long long qb, long long qt,
+                     long long qh, const void* k, long long kb, long long kt, long long kh, const void* v, long long vb,
+                     long long vt, long long vh, const void* o, long long ob, long long ot, long long oh, const float* lse, int B,
+                     int Tq, int Tk, int Hq, int Hk, int D, const int* lengths, const int* query_lengths, int causal,
+                     const int* query_starts, int query_start, float scale, void* dq, void* dk, void* dv, float* workspace,
+                     size_t workspace_floats, rs_stream_t stream);
 
 #ifdef __cplusplus
 }

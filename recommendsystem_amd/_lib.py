@@ -140,6 +140,11 @@ _SIGS = {
     # rotary.hip
     "rs_rotary": [I, C.c_void_p, L, L, L, I, C.c_void_p, L, L, L, I, I, I, I, I, I, C.c_void_p, I, L, L, c_f32p, c_f32p, I, I,
                   C.c_void_p, C.c_void_p, c_i32p, c_stream],
+    # attention.hip
+    "rs_attention_fwd": [I, *[C.c_void_p, L, L, L] * 3, I, I, I, I, I, I, c_i32p, c_i32p, I, c_i32p, I, F, C.c_void_p, c_f32p,
+                         c_f32p, SZ, c_stream],
+    "rs_attention_bwd": [I, *[C.c_void_p, L, L, L] * 5, c_f32p, I, I, I, I, I, I, c_i32p, c_i32p, I, c_i32p, I, F, C.c_void_p,
+                         C.c_void_p, C.c_void_p, c_f32p, SZ, c_stream],
     # shard.hip
     "rs_shard_route": [c_i32p, I, I, c_i64p, I, c_i32p, c_i32p, I, c_i64p, c_i32p, c_i32p, c_stream],
     "rs_shard_gather": [c_i64p, c_i64p, c_i64p, I, I, c_i32p, c_i32p, I, I, I, c_f32p, c_f32p, c_f32p, c_f32p, I, I,
@@ -203,6 +208,8 @@ _PLAIN = {
     "rs_sparse_touched_dot_groups": (I, [I, I]),
     "rs_act_bwd_num_partials": (I, [L]),
     "rs_interact_partial_rows": (I, [I]),
+    "rs_attention_fwd_workspace_floats": (SZ, [I, I, I, I, I, I, I]),
+    "rs_attention_bwd_workspace_floats": (SZ, [I, I, I]),
     "rs_layer_norm_partial_rows": (I, [I, I]),
     "rs_layer_norm_bwd_workspace_floats": (SZ, [I, I]),
     "rs_ffm_bwd_num_partials": (I, [I, I]),

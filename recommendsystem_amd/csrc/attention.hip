@@ -1,0 +1,785 @@
+// Attention over fields, histories and cached keys: forward, backward and single tokens; fp32, bf16 and fp16, heads of up
+// to 128 elements, several query heads to a key head.
+//
+//   z_ij = scale q_i . k_j,  p_ij = exp(z_ij - lse_i) over the keys row i sees,  o_i = sum_j p_ij v_j
+//   delta_i = sum_d do_id o_id,  ds_ij = p_ij (do_i . v_j - delta_i)
+//   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,  dv_j = sum_i p_ij do_i
+// Row i of sample b sees key j where j < lengths[b], i < query_lengths[b] and, causal, j <= i + query_start[b].  A row that
+// sees nothing has o = 0, lse = -inf and no part in any gradient; what lies in keys and rows behind the lengths is never
+// multiplied with anything.
+//
+// One pass over the keys with the running maximum and sum of the softmax; no matrix of scores exists.  All products run on
+// the matrix cores as 32x32 tiles, always "A from LDS, B from registers": the fixed operand of a wave (its 32 query
+// rows, or its 32 keys) stays in registers as columns, tiles of the other one pass through LDS.  The result of such a
+// product holds one column per lane (and its partner lane + 32), 16 rows each, which is the layout the next product
+// wants as its B operand if the contraction runs over the rows in the order the registers hold them: the scores turn into
+// probabilities and go into the next product without leaving their lane.  The transposed A operands of that product
+// (v, k, q, do with the head dimension as rows) are read from the same LDS tile, 16-bit types with the transposing LDS load.
+//   forward   S^T = K Q^T, softmax down the lane's own registers, O^T += V^T P^T
+//   dq        S^T, dP^T = V dO^T, dQ^T += K^T dS^T;  delta is made here and left for the other one
+//   dk, dv    S = Q K^T, dP = dO V^T, dV^T += dO^T P, dK^T += Q^T dS
+// The backward makes the scores twice (14 D instead of 10 D operations per pair) so that every gradient has one owner: no
+// atomics, the same bits every time.  Query heads that share a key head lie next to one another as rows of the forward
+// and dq (row = position * group + head), so a cache is read once for all of them; dk / dv walk over them.
+//
+// Roundings: products of 16-bit operands are exact and summed in fp32; P and dS are rounded to the operands' type for
+// their second product (the matrix cores take equal types; the rounding is a half step per element and averages out over
+// the keys); all statistics, sums and outputs before their last rounding are fp32.
+#include "lowp.h"
+#include "../../include/rs_hip.h"
+
+#pragma clang fp contract(fast)
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+struct Operand {
+    const void* p;
+    long long b, t, h;      // strides in elements
+};
+
+struct AttnArgs {
+    Operand q, k, v, o, go;                  // go: gradient of o
+    void *out, *dq, *dk, *dv;                // contiguous
+    float *lse, *delta;                      // [B, Hq, Tq]
+    const int *len, *qlen, *qstart;          // [B] or null
+    int B, Tq, Tk, Hk, G, D, causal, start;
+    float scale;
+    int tiles, splits;                       // row (key) tiles per (sample, key head); shares of the keys
+    long long units;                         // workgroups with work
+    float *part_o, *part_ml;                 // with splits > 1: [splits, B * Hk, Tq * G, D], lse in base 2 [.., Tq * G]
+    int vec;                                 // 16-byte accesses to q, k, v, o, go
+    int out_vec;                             // four elements at once to the outputs
+};
+
+typedef short rs_s16x4 __attribute__((ext_vector_type(4)));
+
+// Matrix tiles of one element type.  CK: elements of the contraction in one fragment pair; a fragment is 16 bytes a lane.
+template <typename T> struct Mma;
+template <> struct Mma<float> {
+    static constexpr int CK = 8, E = 4;
+    typedef rs_f32x4 V;
+    static __device__ __forceinline__ rs_f32x16 mul(V a, V b, rs_f32x16 c) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
+        return c;
+    }
+};
+template <> struct Mma<__bf16> {
+    static constexpr int CK = 16, E = 8;
+    typedef rs_bf16x8 V;
+    static __device__ __forceinline__ rs_f32x16 mul(V a, V b, rs_f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+};
+template <> struct Mma<_Float16> {
+    static constexpr int CK = 16, E = 8;
+    typedef rs_f16x8 V;
+    static __device__ __forceinline__ rs_f32x16 mul(V a, V b, rs_f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+};
+
+// A tile of R rows in LDS, DP elements and 16 bytes of padding to a row: consecutive rows start 4 banks apart.
+template <typename T, int DP> struct Tile {
+    static constexpr int RS = DP + 16 / (int)sizeof(T);
+    typedef typename Mma<T>::V V;
+
+    // rows row0 + lane % 32, elements of contraction step c
+    static __device__ __forceinline__ V rows(const T* lds, int row0, int c) {
+        const int l = threadIdx.x & 63;
+        return *(const V*)(lds + (row0 + (l & 31)) * RS + c * Mma<T>::CK + (l >> 5) * Mma<T>::E);
+    }
+    // transposed: element col0 + lane % 32 of the rows that the registers of a product hold for contraction step c --
+    // half h of the wave has rows 4h .. 4h+3 of each group of eight
+    static __device__ __forceinline__ V cols(const T* lds, int row0, int col0) {
+        const int l = threadIdx.x & 63;
+        if constexpr (sizeof(T) == 4) {
+            V r;
+            const T* p = lds + (row0 + 4 * (l >> 5)) * RS + col0 + (l & 31);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[i] = p[i * RS];
+            return r;
+        } else {
+            // 16 lanes read 4 rows of 16 elements and get one element of each row
+            const T* p = lds + (row0 + 4 * (l >> 5) + ((l & 15) >> 2)) * RS + col0 + 16 * ((l >> 4) & 1) + 4 * (l & 3);
+            typedef __attribute__((address_space(3))) rs_s16x4* lds_ptr;
+            union { rs_s16x4 s[2]; V v; } r;
+            r.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)p);
+            r.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 8 * RS));
+            return r.v;
+        }
+    }
+};
+
+// E elements from column col of a row of D (zeros behind D, and everywhere when the row has no part).
+template <typename T> __device__ __forceinline__ typename Mma<T>::V fetch(const T* row, int col, int D, int vec, bool live) {
+    typename Mma<T>::V r;
+    constexpr int E = Mma<T>::E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) r[e] = (T)0.f;
+    if (live && col < D) {
+        if (vec) {
+            r = *(const typename Mma<T>::V*)(row + col);
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (col + e < D) r[e] = row[col + e];
+        }
+    }
+    return r;
+}
+
+// A tile's way from memory through registers into LDS: NT lanes, R rows.
+template <typename T, int DP, int R, int NT> struct Stage {
+    static constexpr int E = Mma<T>::E, PER_ROW = DP / E, N = R * PER_ROW / NT;
+    static_assert(R * PER_ROW % NT == 0, "the lanes share a tile evenly");
+    typename Mma<T>::V r[N];
+    __device__ __forceinline__ void load(const T* base, long long row_stride, int row0, int row_end, int D, int vec) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int x = threadIdx.x + i * NT, row = row0 + x / PER_ROW;
+            r[i] = fetch<T>(base + row * row_stride, (x % PER_ROW) * E, D, vec, row < row_end);
+        }
+    }
+    __device__ __forceinline__ void store(T* lds) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int x = threadIdx.x + i * NT;
+            *(typename Mma<T>::V*)(lds + (x / PER_ROW) * Tile<T, DP>::RS + (x % PER_ROW) * E) = r[i];
+        }
+    }
+};
+
+// The registers of contraction step c of a product as the next product's B operand.
+template <typename T> __device__ __forceinline__ typename Mma<T>::V pack(const rs_f32x16& s, int c) {
+    typename Mma<T>::V r;
+#pragma unroll
+    for (int e = 0; e < Mma<T>::E; ++e) r[e] = (T)s[c * Mma<T>::E + e];
+    return r;
+}
+
+__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
+// Row of register i within a 32x32 result.
+__device__ __forceinline__ int reg_row(int i) { return 8 * (i >> 2) + 4 * ((threadIdx.x & 63) >> 5) + (i & 3); }
+
+// Workgroup -> unit of work: ids go round the eight XCDs, so that neighbouring units, which read the same keys, get to
+// one XCD and its L2.
+__device__ __forceinline__ long long unit_of(long long id, long long units) {
+    const long long per = (units + 7) / 8;
+    return (id >> 3) < per ? (id & 7) * per + (id >> 3) : units;
+}
+
+// What a lane's row sees: keys below the result.
+__device__ __forceinline__ int row_limit(const AttnArgs& a, int b, int i) {
+    int lim = a.len ? min(max(a.len[b], 0), a.Tk) : a.Tk;
+    const int rows = a.qlen ? min(a.qlen[b], a.Tq) : a.Tq;
+    if (i >= rows) return 0;
+    if (a.causal) {
+        const long long last = (long long)i + (a.qstart ? a.qstart[b] : a.start) + 1;
+        lim = last < lim ? (last < 0 ? 0 : (int)last) : lim;
+    }
+    return lim;
+}
+
+template <typename T> __device__ __forceinline__ const T* row_ptr(const Operand& x, int b, int t, int h) {
+    return (const T*)x.p + b * x.b + t * x.t + h * x.h;
+}
+
+// Four consecutive elements of an output row.
+template <typename T> __device__ __forceinline__ void store4(T* row, int d, int D, bool vec, const float* v) {
+    if (vec && d + 4 <= D) {
+        if constexpr (sizeof(T) == 4) {
+            *(rs_f32x4*)(row + d) = rs_f32x4{v[0], v[1], v[2], v[3]};
+        } else {
+            typedef T T4 __attribute__((ext_vector_type(4)));
+            *(T4*)(row + d) = T4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (d + e < D) row[d + e] = (T)v[e];
+    }
+}
+
+template <typename T, int DP> constexpr int tile_rows() { return sizeof(T) == 4 && DP == 128 ? 32 : 64; }
+
+// ---- forward -----------------------------------------------------------------------------------------------------
+template <typename T, int DP, int NW, int KT>
+__global__ __launch_bounds__(NW * 64) void attention_fwd_kernel(const AttnArgs a) {
+    constexpr int NT = NW * 64, BM = NW * 32, CK = Mma<T>::CK, E = Mma<T>::E, NC = DP / CK, NB = DP / 32, KB = KT / 32;
+    typedef typename Mma<T>::V V;
+    typedef Tile<T, DP> L;
+    __shared__ __align__(16) T s_k[2][KT * L::RS];
+    __shared__ __align__(16) T s_v[2][KT * L::RS];
+    const long long unit = unit_of(rs_block_id(), a.units);
+    if (unit >= a.units) return;
+    const int split = (int)(unit % a.splits);
+    const long long rest = unit / a.splits;
+    const int tile = a.tiles - 1 - (int)(rest % a.tiles);        // causal: the long rows first
+    const int pair = (int)(rest / a.tiles), b = pair / a.Hk, hk = pair % a.Hk;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const int rows = a.Tq * a.G, row = tile * BM + wave * 32 + (lane & 31);
+    const int i = row / a.G, h = hk * a.G + row % a.G;
+    const bool live = row < rows;
+    const int lim = live ? row_limit(a, b, i) : 0;
+    // keys any row of the workgroup sees, and all live rows of this wave (rows only see more further down)
+    const int last = min(tile * BM + BM, rows) - 1;
+    int end = row_limit(a, b, last / a.G);
+    if (end == 0) {                                               // its last rows may lie behind the sample's
+        const int n = a.qlen ? min(a.qlen[b], a.Tq) : a.Tq;
+        if (n > 0 && n - 1 < last / a.G && n - 1 >= tile * BM / a.G) end = row_limit(a, b, n - 1);
+    }
+    int low = lim;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) low = min(low, __shfl_xor(low, o, 64));
+    low = __builtin_amdgcn_readfirstlane(low);
+    int k0 = 0;
+    if (a.splits > 1) {                                           // this share's whole tiles of them
+        const int per = ((end + KT - 1) / KT + a.splits - 1) / a.splits * KT;
+        k0 = min(split * per, end);
+        end = min(k0 + per, end);
+    }
+
+    V qf[NC];
+    {
+        const T* qr = row_ptr<T>(a.q, b, live ? i : 0, live ? h : 0);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) qf[c] = fetch<T>(qr, c * CK + half * E, a.D, a.vec, live && lim > 0);
+    }
+    rs_f32x16 acc[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[n][e] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    const float scale2 = a.scale * LOG2E;
+    const T* kp = row_ptr<T>(a.k, b, 0, hk);
+    const T* vp = row_ptr<T>(a.v, b, 0, hk);
+    Stage<T, DP, KT, NT> sk, sv;
+    if (k0 < end) {
+        sk.load(kp, a.k.t, k0, end, a.D, a.vec);
+        sv.load(vp, a.v.t, k0, end, a.D, a.vec);
+    }
+    for (int buf = 0; k0 < end; k0 += KT, buf ^= 1) {
+        sk.store(s_k[buf]);
+        sv.store(s_v[buf]);
+        __syncthreads();       // the other buffer's readers are past it: they stored this one after their last read
+        if (k0 + KT < end) {
+            sk.load(kp, a.k.t, k0 + KT, end, a.D, a.vec);
+            sv.load(vp, a.v.t, k0 + KT, end, a.D, a.vec);
+        }
+        rs_f32x16 s[KB];
+#pragma unroll
+        for (int n = 0; n < KB; ++n) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[n][e] = 0.f;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) s[n] = Mma<T>::mul(L::rows(s_k[buf], n * 32, c), qf[c], s[n]);
+        }
+        if (k0 + KT > low) {
+#pragma unroll
+            for (int n = 0; n < KB; ++n)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (k0 + n * 32 + reg_row(e) >= lim) s[n][e] = -INFINITY;
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int n = 0; n < KB; ++n)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) top = fmaxf(top, s[n][e]);
+        top = fmaxf(top, other_half(top)) * scale2;
+        const float m_new = fmaxf(m, top);
+        const float base = m_new == -INFINITY ? 0.f : m_new;     // nothing seen yet: exp2(-inf - 0) = 0 throughout
+        const float alpha = exp2f(m - base);
+        m = m_new;
+        float sum = 0.f;
+#pragma unroll
+        for (int n = 0; n < KB; ++n)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                s[n][e] = __builtin_amdgcn_exp2f(s[n][e] * scale2 - base);
+                sum += s[n][e];
+            }
+        l = l * alpha + sum;                                      // this half's keys only
+        if (__any(alpha != 1.f)) {
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[n][e] *= alpha;
+        }
+#pragma unroll
+        for (int n = 0; n < KB; ++n)
+#pragma unroll
+            for (int c = 0; c < 32 / CK; ++c) {
+                const V p = pack<T>(s[n], c);
+#pragma unroll
+                for (int d = 0; d < NB; ++d) acc[d] = Mma<T>::mul(L::cols(s_v[buf], n * 32 + c * CK, d * 32), p, acc[d]);
+            }
+    }
+    if (!live) return;
+    l += other_half(l);
+    const float inv = l == 0.f ? 0.f : 1.f / l;                   // nothing seen: zeros (a NaN stays one)
+    if (a.splits > 1) {
+        const long long at = ((long long)split * a.B * a.Hk + pair) * rows + row;
+        if (half == 0) a.part_ml[at] = l == 0.f ? -INFINITY : m + log2f(l);
+#pragma unroll
+        for (int d = 0; d < NB; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                float o[4];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) o[x] = acc[d][e + x] * inv;
+                store4<float>(a.part_o + at * a.D, d * 32 + reg_row(e), a.D, a.D % 4 == 0, o);
+            }
+        return;
+    }
+    if (a.lse && half == 0) a.lse[((long long)b * a.Hk * a.G + h) * a.Tq + i] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+    T* out = (T*)a.out + (((long long)b * a.Tq + i) * a.Hk * a.G + h) * a.D;
+#pragma unroll
+    for (int d = 0; d < NB; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            float o[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o[x] = acc[d][e + x] * inv;
+            store4<T>(out, d * 32 + reg_row(e), a.D, a.out_vec, o);
+        }
+}
+
+// Joins the shares of a row: weights exp2(lse_s - max) over their sum.  A wave to a row.
+template <typename T> __global__ __launch_bounds__(256) void attention_join_kernel(const AttnArgs a) {
+    const long long rows = (long long)a.Tq * a.G, all = rows * a.B * a.Hk;
+    const long long at = rs_block_id() * 4 + (threadIdx.x >> 6);
+    if (at >= all) return;
+    const int lane = threadIdx.x & 63;
+    const long long pair = at / rows;
+    const int row = (int)(at - pair * rows), i = row / a.G, b = (int)(pair / a.Hk), h = (int)(pair % a.Hk) * a.G + row % a.G;
+    float m = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[s * all + at]);
+    const float base = m == -INFINITY ? 0.f : m;
+    float l = 0.f, o0 = 0.f, o1 = 0.f;
+    for (int s = 0; s < a.splits; ++s) {
+        const float w = exp2f(a.part_ml[s * all + at] - base);
+        const float* p = a.part_o + (s * all + at) * a.D;
+        l += w;
+        if (w != 0.f) {
+            if (lane < a.D) o0 += w * p[lane];
+            if (lane + 64 < a.D) o1 += w * p[lane + 64];
+        }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T* out = (T*)a.out + (((long long)b * a.Tq + i) * a.Hk * a.G + h) * a.D;
+    if (lane < a.D) out[lane] = (T)(o0 * inv);
+    if (lane + 64 < a.D) out[lane + 64] = (T)(o1 * inv);
+    if (a.lse && lane == 0) a.lse[((long long)b * a.Hk * a.G + h) * a.Tq + i] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+}
+
+// ---- dq, and delta for the other gradients -----------------------------------------------------------------------------
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(NW * 64) void attention_dq_kernel(const AttnArgs a) {
+    constexpr int KT = tile_rows<T, DP>();
+    constexpr int NT = NW * 64, BM = NW * 32, CK = Mma<T>::CK, E = Mma<T>::E, NC = DP / CK, NB = DP / 32, KB = KT / 32;
+    typedef typename Mma<T>::V V;
+    typedef Tile<T, DP> L;
+    __shared__ __align__(16) T s_k[2][KT * L::RS];
+    __shared__ __align__(16) T s_v[2][KT * L::RS];
+    const long long unit = unit_of(rs_block_id(), a.units);
+    if (unit >= a.units) return;
+    const int tile = a.tiles - 1 - (int)(unit % a.tiles);
+    const int pair = (int)(unit / a.tiles), b = pair / a.Hk, hk = pair % a.Hk;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const int rows = a.Tq * a.G, row = tile * BM + wave * 32 + (lane & 31);
+    const int i = row / a.G, h = hk * a.G + row % a.G;
+    const bool live = row < rows;
+    const int lim = live ? row_limit(a, b, i) : 0;
+    const int last = min(tile * BM + BM, rows) - 1;
+    int end = row_limit(a, b, last / a.G);
+    if (end == 0) {
+        const int n = a.qlen ? min(a.qlen[b], a.Tq) : a.Tq;
+        if (n > 0 && n - 1 < last / a.G && n - 1 >= tile * BM / a.G) end = row_limit(a, b, n - 1);
+    }
+    int low = lim;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) low = min(low, __shfl_xor(low, o, 64));
+    low = __builtin_amdgcn_readfirstlane(low);
+
+    V qf[NC], gf[NC];
+    float delta = 0.f, lse2 = INFINITY;
+    {
+        const bool has = live && lim > 0;
+        const T* qr = row_ptr<T>(a.q, b, live ? i : 0, live ? h : 0);
+        const T* gr = row_ptr<T>(a.go, b, live ? i : 0, live ? h : 0);
+        const T* orow = row_ptr<T>(a.o, b, live ? i : 0, live ? h : 0);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            qf[c] = fetch<T>(qr, c * CK + half * E, a.D, a.vec, has);
+            gf[c] = fetch<T>(gr, c * CK + half * E, a.D, a.vec, has);
+            const V of = fetch<T>(orow, c * CK + half * E, a.D, a.vec, has);
+#pragma unroll
+            for (int e = 0; e < E; ++e) delta += (float)gf[c][e] * (float)of[e];
+        }
+        delta += other_half(delta);
+        const long long at = ((long long)b * a.Hk * a.G + h) * a.Tq + i;
+        if (has) lse2 = a.lse[at] * LOG2E;
+        if (live && half == 0) a.delta[at] = delta;
+    }
+    rs_f32x16 acc[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[n][e] = 0.f;
+    const float scale2 = a.scale * LOG2E;
+    const T* kp = row_ptr<T>(a.k, b, 0, hk);
+    const T* vp = row_ptr<T>(a.v, b, 0, hk);
+    Stage<T, DP, KT, NT> sk, sv;
+    if (0 < end) {
+        sk.load(kp, a.k.t, 0, end, a.D, a.vec);
+        sv.load(vp, a.v.t, 0, end, a.D, a.vec);
+    }
+    for (int k0 = 0, buf = 0; k0 < end; k0 += KT, buf ^= 1) {
+        sk.store(s_k[buf]);
+        sv.store(s_v[buf]);
+        __syncthreads();
+        if (k0 + KT < end) {
+            sk.load(kp, a.k.t, k0 + KT, end, a.D, a.vec);
+            sv.load(vp, a.v.t, k0 + KT, end, a.D, a.vec);
+        }
+#pragma unroll
+        for (int n = 0; n < KB; ++n) {
+            rs_f32x16 s, dp;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                s = Mma<T>::mul(L::rows(s_k[buf], n * 32, c), qf[c], s);
+                dp = Mma<T>::mul(L::rows(s_v[buf], n * 32, c), gf[c], dp);
+            }
+            if (k0 + n * 32 + 32 > low) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (k0 + n * 32 + reg_row(e) >= lim) s[e] = -INFINITY;
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(s[e] * scale2 - lse2) * (dp[e] - delta);
+#pragma unroll
+            for (int c = 0; c < 32 / CK; ++c) {
+                const V p = pack<T>(s, c);
+#pragma unroll
+                for (int d = 0; d < NB; ++d) acc[d] = Mma<T>::mul(L::cols(s_k[buf], n * 32 + c * CK, d * 32), p, acc[d]);
+            }
+        }
+    }
+    if (!live) return;
+    T* out = (T*)a.dq + (((long long)b * a.Tq + i) * a.Hk * a.G + h) * a.D;
+#pragma unroll
+    for (int d = 0; d < NB; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            float o[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o[x] = acc[d][e + x] * a.scale;
+            store4<T>(out, d * 32 + reg_row(e), a.D, a.out_vec, o);
+        }
+}
+
+// ---- dk and dv -----------------------------------------------------------------------------------------------------------
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(NW * 64) void attention_dkv_kernel(const AttnArgs a) {
+    constexpr int RT = tile_rows<T, DP>();
+    constexpr int NT = NW * 64, BN = NW * 32, CK = Mma<T>::CK, E = Mma<T>::E, NC = DP / CK, NB = DP / 32, RB = RT / 32;
+    typedef typename Mma<T>::V V;
+    typedef Tile<T, DP> L;
+    __shared__ __align__(16) T s_q[2][RT * L::RS];
+    __shared__ __align__(16) T s_g[2][RT * L::RS];
+    __shared__ __align__(16) float s_lse[2][RT], s_delta[2][RT];
+    __shared__ __align__(16) int s_lim[2][RT];
+    const long long unit = unit_of(rs_block_id(), a.units);
+    if (unit >= a.units) return;
+    const int tile = (int)(unit % a.tiles);                       // causal: the first keys are seen by the most rows
+    const int pair = (int)(unit / a.tiles), b = pair / a.Hk, hk = pair % a.Hk;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const int key = tile * BN + wave * 32 + (lane & 31);
+    const int len = a.len ? min(max(a.len[b], 0), a.Tk) : a.Tk;
+    const int qrows = a.qlen ? min(max(a.qlen[b], 0), a.Tq) : a.Tq;
+    int begin = 0;                                                // first row that sees a key of this workgroup
+    if (a.causal) {
+        const long long f = (long long)tile * BN - (a.qstart ? a.qstart[b] : a.start);
+        begin = f <= 0 ? 0 : f >= qrows ? qrows : (int)f;
+    }
+    const int stop = tile * BN < len ? qrows : 0;
+
+    V kf[NC], vf[NC];
+    {
+        const bool has = key < len;
+        const T* kr = row_ptr<T>(a.k, b, has ? key : 0, hk);
+        const T* vr = row_ptr<T>(a.v, b, has ? key : 0, hk);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            kf[c] = fetch<T>(kr, c * CK + half * E, a.D, a.vec, has);
+            vf[c] = fetch<T>(vr, c * CK + half * E, a.D, a.vec, has);
+        }
+    }
+    rs_f32x16 dk[NB], dv[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dk[n][e] = dv[n][e] = 0.f;
+    const float scale2 = a.scale * LOG2E;
+    Stage<T, DP, RT, NT> sq, sg;
+    float r_lse = INFINITY, r_delta = 0.f;
+    int r_lim = 0;
+    const int per_head = begin < stop ? (stop - begin + RT - 1) / RT : 0, turns = per_head * a.G;
+    // turn -> (head of the group, row tile)
+    auto load = [&](int turn) {
+        const int h = hk * a.G + turn / per_head, r0 = begin + turn % per_head * RT;
+        sq.load(row_ptr<T>(a.q, b, 0, h), a.q.t, r0, stop, a.D, a.vec);
+        sg.load(row_ptr<T>(a.go, b, 0, h), a.go.t, r0, stop, a.D, a.vec);
+        if (threadIdx.x < RT) {
+            const int i = r0 + threadIdx.x;
+            r_lim = i < stop ? row_limit(a, b, i) : 0;
+            const long long at = ((long long)b * a.Hk * a.G + h) * a.Tq + i;
+            r_lse = r_lim > 0 ? a.lse[at] * LOG2E : INFINITY;     // a row that sees nothing: exp2(-inf) = 0
+            r_delta = r_lim > 0 ? a.delta[at] : 0.f;
+        }
+    };
+    if (turns > 0) load(0);
+    for (int turn = 0, buf = 0; turn < turns; ++turn, buf ^= 1) {
+        sq.store(s_q[buf]);
+        sg.store(s_g[buf]);
+        if (threadIdx.x < RT) {
+            s_lse[buf][threadIdx.x] = r_lse;
+            s_delta[buf][threadIdx.x] = r_delta;
+            s_lim[buf][threadIdx.x] = r_lim;
+        }
+        __syncthreads();
+        if (turn + 1 < turns) load(turn + 1);
+#pragma unroll
+        for (int n = 0; n < RB; ++n) {
+            rs_f32x16 s, dp;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                s = Mma<T>::mul(L::rows(s_q[buf], n * 32, c), kf[c], s);
+                dp = Mma<T>::mul(L::rows(s_g[buf], n * 32, c), vf[c], dp);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int r = n * 32 + reg_row(e);
+                const rs_f32x4 ls = *(const rs_f32x4*)&s_lse[buf][r], de = *(const rs_f32x4*)&s_delta[buf][r];
+                const int4 li = *(const int4*)&s_lim[buf][r];
+                const int lim[4] = {li.x, li.y, li.z, li.w};
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const bool seen = key < lim[x];               // selected, not multiplied: an unseen key may hold anything
+                    const float p = seen ? __builtin_amdgcn_exp2f(s[e + x] * scale2 - ls[x]) : 0.f;
+                    s[e + x] = p;
+                    dp[e + x] = seen ? p * (dp[e + x] - de[x]) : 0.f;
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 32 / CK; ++c) {
+                const V p = pack<T>(s, c), ds = pack<T>(dp, c);
+#pragma unroll
+                for (int d = 0; d < NB; ++d) {
+                    dv[d] = Mma<T>::mul(L::cols(s_g[buf], n * 32 + c * CK, d * 32), p, dv[d]);
+                    dk[d] = Mma<T>::mul(L::cols(s_q[buf], n * 32 + c * CK, d * 32), ds, dk[d]);
+                }
+            }
+        }
+    }
+    if (key >= a.Tk) return;
+    const long long at = (((long long)b * a.Tk + key) * a.Hk + hk) * a.D;
+#pragma unroll
+    for (int d = 0; d < NB; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            float o[4], u[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                o[x] = dk[d][e + x] * a.scale;
+                u[x] = dv[d][e + x];
+            }
+            store4<T>((T*)a.dk + at, d * 32 + reg_row(e), a.D, a.out_vec, o);
+            store4<T>((T*)a.dv + at, d * 32 + reg_row(e), a.D, a.out_vec, u);
+        }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------
+inline int padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+inline int waves_for(long long rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : 4; }
+inline int key_tile(int dtype, int D, int nw) { return nw == 1 || (dtype == RS_F32 && padded(D) == 128) ? 32 : 64; }
+
+// Shares of the keys: few rows leave most of the chip idle, so the keys of a sample are split until there are about
+// eight waves for every CU, but no share is shorter than four tiles.
+int splits_for(int dtype, int B, int Tq, int Tk, int Hk, int G, int D) {
+    const long long rows = (long long)Tq * G;
+    const int nw = waves_for(rows);
+    const long long units = (long long)B * Hk * ((rows + nw * 32 - 1) / (nw * 32));
+    const long long want = 2048 / nw / units, most = Tk / (4 * key_tile(dtype, D, nw));
+    const long long s = want < most ? want : most;
+    return s < 1 ? 1 : s > 64 ? 64 : (int)s;
+}
+
+template <typename T, int DP, int NW> int launch_fwd(const AttnArgs& a, hipStream_t stream) {
+    constexpr int KT = NW == 1 ? 32 : tile_rows<T, DP>();
+    const dim3 grid = rs_grid((a.units + 7) / 8 * 8);
+    hipLaunchKernelGGL((attention_fwd_kernel<T, DP, NW, KT>), grid, dim3(NW * 64), 0, stream, a);
+    RS_CHECK_LAUNCH("rs_attention_fwd");
+    if (a.splits > 1) {
+        hipLaunchKernelGGL((attention_join_kernel<T>), rs_grid(rs_cdiv((long long)a.B * a.Hk * a.Tq * a.G, 4)), dim3(256), 0, stream, a);
+        RS_CHECK_LAUNCH("rs_attention_fwd");
+    }
+    return RS_OK;
+}
+template <typename T, int DP> int launch_fwd(const AttnArgs& a, int nw, hipStream_t stream) {
+    return nw == 1 ? launch_fwd<T, DP, 1>(a, stream) : nw == 2 ? launch_fwd<T, DP, 2>(a, stream) : launch_fwd<T, DP, 4>(a, stream);
+}
+template <typename T> int launch_fwd(const AttnArgs& a, int nw, hipStream_t stream) {
+    const int dp = padded(a.D);
+    return dp == 32 ? launch_fwd<T, 32>(a, nw, stream) : dp == 64 ? launch_fwd<T, 64>(a, nw, stream) : launch_fwd<T, 128>(a, nw, stream);
+}
+
+template <typename T, int DP, int NW> int launch_dq(AttnArgs a, hipStream_t stream) {
+    a.tiles = rs_cdiv((long long)a.Tq * a.G, NW * 32);
+    a.units = (long long)a.B * a.Hk * a.tiles;
+    hipLaunchKernelGGL((attention_dq_kernel<T, DP, NW>), rs_grid((a.units + 7) / 8 * 8), dim3(NW * 64), 0, stream, a);
+    RS_CHECK_LAUNCH("rs_attention_bwd");
+    return RS_OK;
+}
+template <typename T, int DP, int NW> int launch_dkv(AttnArgs a, hipStream_t stream) {
+    a.tiles = rs_cdiv(a.Tk, NW * 32);
+    a.units = (long long)a.B * a.Hk * a.tiles;
+    hipLaunchKernelGGL((attention_dkv_kernel<T, DP, NW>), rs_grid((a.units + 7) / 8 * 8), dim3(NW * 64), 0, stream, a);
+    RS_CHECK_LAUNCH("rs_attention_bwd");
+    return RS_OK;
+}
+template <typename T, int DP> int launch_bwd(const AttnArgs& a, hipStream_t stream) {
+    int rc = RS_OK;
+    if (a.Tq > 0) rc = (long long)a.Tq * a.G <= 64 ? launch_dq<T, DP, 2>(a, stream) : launch_dq<T, DP, 4>(a, stream);
+    if (rc == RS_OK && a.Tk > 0) rc = a.Tk <= 64 ? launch_dkv<T, DP, 2>(a, stream) : launch_dkv<T, DP, 4>(a, stream);
+    return rc;
+}
+template <typename T> int launch_bwd(const AttnArgs& a, hipStream_t stream) {
+    const int dp = padded(a.D);
+    return dp == 32 ? launch_bwd<T, 32>(a, stream) : dp == 64 ? launch_bwd<T, 64>(a, stream) : launch_bwd<T, 128>(a, stream);
+}
+
+bool shape_ok(const char* who, int dtype, int B, int Tq, int Tk, int Hq, int Hk, int D, float scale) {
+    if (!(dtype == RS_F32 || dtype == RS_BF16 || dtype == RS_F16)) {
+        rs_set_error("%s: type %d not served", who, dtype);
+        return false;
+    }
+    if (B < 0 || Tq < 0 || Tk < 0 || Hk < 1 || Hq < Hk || Hq % Hk || D < 1 || D > 128) {
+        rs_set_error("%s: bad shape B=%d Tq=%d Tk=%d Hq=%d Hk=%d D=%d (D <= 128, Hq a multiple of Hk)", who, B, Tq, Tk, Hq, Hk, D);
+        return false;
+    }
+    if (!(scale > 0.f) || scale > 1e30f) {
+        rs_set_error("%s: scale must be positive and finite", who);
+        return false;
+    }
+    // rows and workgroups are counted in 32 bits
+    if ((long long)Tq * (Hq / Hk) > (1 << 30) || Tk > (1 << 30) || (long long)B * Hq * ((Tq > Tk ? Tq : Tk) / 32 + 1) > (1 << 30)) {
+        rs_set_error("%s: too large", who);
+        return false;
+    }
+    return true;
+}
+
+bool operand_vec(const Operand& x, int dtype) {
+    const int e = 16 / rs_elem_bytes(dtype);
+    return !x.p || (rs_aligned16(x.p) && x.b % e == 0 && x.t % e == 0 && x.h % e == 0);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t rs_attention_fwd_workspace_floats(int dtype, int B, int Tq, int Tk, int Hq, int Hk, int D) {
+    if (B <= 0 || Tq <= 0 || Tk <= 0 || Hk < 1 || Hq < Hk || Hq % Hk || D < 1 || D > 128) return 0;
+    const int s = splits_for(dtype, B, Tq, Tk, Hk, Hq / Hk, D);
+    return s == 1 ? 0 : (size_t)s * B * Tq * Hq * (D + 1);
+}
+
+int rs_attention_fwd(int dtype, const void* q, long long qb, long long qt, long long qh, const void* k, long long kb, long long kt,
+                     long long kh, const void* v, long long vb, long long vt, long long vh, int B, int Tq, int Tk, int Hq, int Hk,
+                     int D, const int* lengths, const int* query_lengths, int causal, const int* query_starts, int query_start,
+                     float scale, void* o, float* lse, float* workspace, size_t workspace_floats, rs_stream_t stream) {
+    if (!shape_ok("rs_attention_fwd", dtype, B, Tq, Tk, Hq, Hk, D, scale)) return RS_ERR_ARG;
+    if (B == 0 || Tq == 0) return RS_OK;
+    RS_CHECK_ARG(q && o && (Tk == 0 || (k && v)), "rs_attention_fwd: null argument");
+    AttnArgs a = {};
+    a.q = {q, qb, qt, qh};
+    a.k = {k, kb, kt, kh};
+    a.v = {v, vb, vt, vh};
+    a.out = o;
+    a.lse = lse;
+    a.len = lengths;
+    a.qlen = query_lengths;
+    a.qstart = query_starts;
+    a.B = B, a.Tq = Tq, a.Tk = Tk, a.Hk = Hk, a.G = Hq / Hk, a.D = D, a.causal = causal != 0, a.start = query_start;
+    a.scale = scale;
+    a.vec = D % (16 / rs_elem_bytes(dtype)) == 0 && operand_vec(a.q, dtype) && operand_vec(a.k, dtype) && operand_vec(a.v, dtype);
+    a.out_vec = D % 4 == 0 && rs_aligned16(o);
+    const long long rows = (long long)Tq * a.G;
+    const int nw = waves_for(rows);
+    a.tiles = rs_cdiv(rows, nw * 32);
+    a.splits = Tk > 0 ? splits_for(dtype, B, Tq, Tk, Hk, a.G, D) : 1;
+    a.units = (long long)B * Hk * a.tiles * a.splits;
+    if (a.splits > 1) {
+        const size_t need = rs_attention_fwd_workspace_floats(dtype, B, Tq, Tk, Hq, Hk, D);
+        if (!workspace || workspace_floats < need) {
+            rs_set_error("rs_attention_fwd: workspace of %zu floats, %zu needed", workspace_floats, need);
+            return RS_ERR_WORKSPACE;
+        }
+        RS_CHECK_ARG(rs_aligned16(workspace), "rs_attention_fwd: workspace must be aligned to 16 bytes");
+        a.part_o = workspace;
+        a.part_ml = workspace + (size_t)a.splits * B * Tq * Hq * D;
+    }
+    if (dtype == RS_F32) return launch_fwd<float>(a, nw, stream);
+    if (dtype == RS_BF16) return launch_fwd<__bf16>(a, nw, stream);
+    return launch_fwd<_Float16>(a, nw, stream);
+}
+
+size_t rs_attention_bwd_workspace_floats(int B, int Tq, int Hq) { return B > 0 && Tq > 0 && Hq > 0 ? (size_t)B * Tq * Hq : 0; }
+
+int rs_attention_bwd(int dtype, const void* go, long long gb, long long gt, long long gh, const void* q, long long qb, long long qt,
+                     long long qh, const void* k, long long kb, long long kt, long long kh, const void* v, long long vb,
+                     long long vt, long long vh, const void* o, long long ob, long long ot, long long oh, const float* lse, int B,
+                     int Tq, int Tk, int Hq, int Hk, int D, const int* lengths, const int* query_lengths, int causal,
+                     const int* query_starts, int query_start, float scale, void* dq, void* dk, void* dv, float* workspace,
+                     size_t workspace_floats, rs_stream_t stream) {
+    if (!shape_ok("rs_attention_bwd", dtype, B, Tq, Tk, Hq, Hk, D, scale)) return RS_ERR_ARG;
+    if (B == 0 || (Tq == 0 && Tk == 0)) return RS_OK;
+    RS_CHECK_ARG((Tq == 0 || (go && q && o && lse && dq)) && (Tk == 0 || (k && v && dk && dv)), "rs_attention_bwd: null argument");
+    if (Tq > 0 && (!workspace || workspace_floats < rs_attention_bwd_workspace_floats(B, Tq, Hq))) {
+        rs_set_error("rs_attention_bwd: workspace of %zu floats, %zu needed", workspace_floats, rs_attention_bwd_workspace_floats(B, Tq, Hq));
+        return RS_ERR_WORKSPACE;
+    }
+    AttnArgs a = {};
+    a.q = {q, qb, qt, qh};
+    a.k = {k, kb, kt, kh};
+    a.v = {v, vb, vt, vh};
+    a.o = {o, ob, ot, oh};
+    a.go = {go, gb, gt, gh};
+    a.dq = dq, a.dk = dk, a.dv = dv;
+    a.lse = (float*)lse;
+    a.delta = workspace;
+    a.len = lengths;
+    a.qlen = query_lengths;
+    a.qstart = query_starts;
+    a.B = B, a.Tq = Tq, a.Tk = Tk, a.Hk = Hk, a.G = Hq / Hk, a.D = D, a.causal = causal != 0, a.start = query_start;
+    a.scale = scale;
+    a.splits = 1;
+    a.vec = D % (16 / rs_elem_bytes(dtype)) == 0 && operand_vec(a.q, dtype) && operand_vec(a.k, dtype) && operand_vec(a.v, dtype) &&
+            operand_vec(a.o, dtype) && operand_vec(a.go, dtype);
+    a.out_vec = D % 4 == 0 && rs_aligned16(dq) && rs_aligned16(dk) && rs_aligned16(dv);
+    if (dtype == RS_F32) return launch_bwd<float>(a, stream);
+    if (dtype == RS_BF16) return launch_bwd<__bf16>(a, stream);
+    return launch_bwd<_Float16>(a, stream);
+}
+
+}  // extern "C"

@@ -4,6 +4,7 @@
     CrossNetwork                model/DCN/DCN.py:16-17, 48-52
     nfm_bi_interaction          model/NFM/NFM.py:42-44
     AttentionPooling            model/AFM/AFM.py:19-26, 36-42, 47-56
+    attention                   every element attends to every other; no counterpart in the reference
     FieldAwareTables            model/FFM/FFM.py:21-23, 43-62
 
 Forward and backward both run in librs_hip.so; nothing here falls back to torch arithmetic.
@@ -12,6 +13,7 @@ from __future__ import annotations
 
 import torch
 from torch import nn
+from torch.autograd.function import once_differentiable
 
 from . import functional as Fn
 from . import ops
@@ -203,6 +205,37 @@ class AttentionPooling(nn.Module):
     def forward(self, emb):
         a0, a2 = self.attention[0], self.attention[2]
         return _AFMFn.apply(emb, a0.weight, a0.bias, a2.weight, self.p.weight, self.p.bias)
+
+
+# -------------------------------------------------------------------------------------------------
+# attention among fields, or of queries over a history
+# -------------------------------------------------------------------------------------------------
+class _AttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, lengths, query_lengths, causal, query_start, scale):
+        how = dict(lengths=lengths, query_lengths=query_lengths, causal=causal, query_start=query_start, scale=scale)
+        need = any(ctx.needs_input_grad[:3])
+        o, lse = ops.attention_fwd(q, k, v, want_lse=need, **how)
+        if need:
+            ctx.save_for_backward(q, k, v, o, lse, *(t for t in (lengths, query_lengths, query_start) if isinstance(t, torch.Tensor)))
+            ctx.how = {n: (None if isinstance(t, torch.Tensor) else t) for n, t in how.items()}
+            ctx.vectors = [n for n in ("lengths", "query_lengths", "query_start") if isinstance(how[n], torch.Tensor)]
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do):
+        q, k, v, o, lse, *vectors = ctx.saved_tensors
+        grads = ops.attention_bwd(do, q, k, v, o, lse, **{**ctx.how, **dict(zip(ctx.vectors, vectors))})
+        return (*(g if n else None for g, n in zip(grads, ctx.needs_input_grad)), None, None, None, None, None)
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths=None, query_lengths=None, causal: bool = False,
+              query_start=None, scale=None) -> torch.Tensor:
+    """Softmax attention [B, Tq, Hq, D] x [B, Tk, Hk, D] -> [B, Tq, Hq, D] with its gradients (ops.attention_fwd has the
+    arguments).  emb [B, F, d] viewed as [B, F, heads, d / heads] lets a sample's fields attend to one another; a padded
+    batch of histories passes its lengths twice, as keys' and as queries'."""
+    return _AttentionFn.apply(q, k, v, lengths, query_lengths, causal, query_start, scale)
 
 
 # -------------------------------------------------------------------------------------------------

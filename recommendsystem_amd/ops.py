@@ -1768,7 +1768,7 @@ def axpy(a: float, x: torch.Tensor, y: torch.Tensor):
 
 
 # ---------------------------------------------------------------------------------------------
-# sequence operators: layer norm with a residual stream, rotary positions (fp32 / bf16 / fp16)
+# sequence operators: layer norm with a residual stream, rotary positions, attention (fp32 / bf16 / fp16)
 # ---------------------------------------------------------------------------------------------
 _ELEM_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
@@ -1965,3 +1965,85 @@ def rotary(table: RotaryTable, positions: torch.Tensor, q: torch.Tensor, k: Opti
              int(table.interleaved), ptr(positions), int(positions.dtype == torch.int64), pb, pt, ptr(table.cos), ptr(table.sin),
              table.max_positions, int(inverse), ptr(qo), ptr(ko), ptr(table.err_flag))
     return qo if k is None else (qo, ko)
+
+
+def _attention_args(q, k, v, lengths, query_lengths, causal, query_start, scale):
+    """Checks shared by both directions: (q, k, v, dims, device vectors, start, scale)."""
+    code = _elem_code(q, "attention")
+    q = _heads_view(q, "q")
+    k = _heads_view(k, "k", dtype=q.dtype)
+    v = _heads_view(v, "v", k.shape, q.dtype)
+    B, Tq, Hq, D = q.shape
+    Tk, Hk = k.shape[1], k.shape[2]
+    if k.shape[0] != B or k.shape[3] != D:
+        raise RSError(f"attention: k {tuple(k.shape)} does not go with q {tuple(q.shape)}")
+    if not 1 <= D <= 128 or Hk < 1 or Hq < Hk or Hq % Hk:
+        raise RSError(f"attention: heads of 1..128 elements and query heads a multiple of key heads are served, got "
+                      f"{Hq} and {Hk} heads of {D}")
+    for name, t in (("lengths", lengths), ("query_lengths", query_lengths)):
+        if t is not None:
+            _chk_vector(t, name, B)
+    starts, start = None, Tk - Tq
+    if isinstance(query_start, torch.Tensor):
+        _chk_vector(query_start, "query_start", B)
+        starts = query_start
+    elif query_start is not None:
+        start = int(query_start)
+    if not -0x40000000 <= start <= 0x40000000:
+        raise RSError(f"attention: query_start {start} is out of range")
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale <= 1e30:
+        raise RSError(f"attention: scale must be positive and finite, got {scale}")
+    dev = _same_device(("q", q), ("k", k), ("v", v), ("lengths", lengths), ("query_lengths", query_lengths), ("query_start", starts))
+    return code, q, k, v, (B, Tq, Tk, Hq, Hk, D), (ptr(lengths), ptr(query_lengths), int(bool(causal)), ptr(starts), start, scale), dev
+
+
+def _chk_vector(t: torch.Tensor, name: str, n: int):
+    if t.dtype != torch.int32 or tuple(t.shape) != (n,) or not t.is_contiguous():
+        raise RSError(f"attention: {name} must be a contiguous int32 vector of {n}, got {t.dtype} {tuple(t.shape)}")
+
+
+def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: Optional[torch.Tensor] = None,
+                  query_lengths: Optional[torch.Tensor] = None, causal: bool = False, query_start=None,
+                  scale: Optional[float] = None, want_lse: bool = True):
+    """softmax(scale q k^T over the visible keys) v: q [B, Tq, Hq, D], k and v [B, Tk, Hk, D], D <= 128, Hq a multiple of Hk
+    (neighbouring query heads share a key head); float32, bfloat16 or float16; strides as they come, only the last
+    dimension has to be contiguous (views of one projection, or a cache longer than its contents, are read in place).
+
+    Row i of sample b sees key j where j < lengths[b] and i < query_lengths[b] (int32 [B], None: all) and, causal,
+    j <= i + query_start: an int, an int32 [B], or None for Tk - Tq, which lines up the last row with the last key.  Rows
+    that see nothing get zeros (lse -inf), and what lies behind the lengths is never used, whatever it holds.
+    scale: D ** -0.5 by default, positive.  Returns (o, lse): o [B, Tq, Hq, D], lse [B, Hq, Tq] float32 or None."""
+    code, q, k, v, (B, Tq, Tk, Hq, Hk, D), how, dev = _attention_args(q, k, v, lengths, query_lengths, causal, query_start, scale)
+    o = torch.empty((B, Tq, Hq, D), dtype=q.dtype, device=dev)
+    lse = torch.empty((B, Hq, Tq), dtype=torch.float32, device=dev) if want_lse else None
+    floats = _lib.lib().rs_attention_fwd_workspace_floats(code, B, Tq, Tk, Hq, Hk, D)
+    # per call: two captured graphs, or two streams, never share the partial results
+    work = torch.empty(floats, dtype=torch.float32, device=dev) if floats else None
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
+    _call_on(dev, "rs_attention_fwd", code, ptr(q), qs[0], qs[1], qs[2], ptr(k), ks[0], ks[1], ks[2], ptr(v), vs[0], vs[1], vs[2],
+             B, Tq, Tk, Hq, Hk, D, *how, ptr(o), ptr(lse), ptr(work), floats)
+    return o, lse
+
+
+def attention_bwd(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor,
+                  lengths: Optional[torch.Tensor] = None, query_lengths: Optional[torch.Tensor] = None, causal: bool = False,
+                  query_start=None, scale: Optional[float] = None):
+    """Gradients (dq, dk, dv) of attention_fwd's o from do, with the same arguments and the forward's o and lse; the
+    probabilities are computed again.  Shared key heads get the sum over their query heads.  No atomics: the same bits
+    every time."""
+    code, q, k, v, (B, Tq, Tk, Hq, Hk, D), how, _ = _attention_args(q, k, v, lengths, query_lengths, causal, query_start, scale)
+    do = _heads_view(do, "do", q.shape, q.dtype)
+    o = _heads_view(o, "o", q.shape, q.dtype)
+    _chk(lse, torch.float32, "lse", (B, Hq, Tq))
+    dev = _same_device(("q", q), ("do", do), ("o", o), ("lse", lse))
+    dq = torch.empty((B, Tq, Hq, D), dtype=q.dtype, device=dev)
+    dk = torch.empty((B, Tk, Hk, D), dtype=q.dtype, device=dev)
+    dv = torch.empty((B, Tk, Hk, D), dtype=q.dtype, device=dev)
+    floats = _lib.lib().rs_attention_bwd_workspace_floats(B, Tq, Hq)
+    work = torch.empty(max(floats, 1), dtype=torch.float32, device=dev)
+    gs, qs, ks, vs, os_ = do.stride(), q.stride(), k.stride(), v.stride(), o.stride()
+    _call_on(dev, "rs_attention_bwd", code, ptr(do), gs[0], gs[1], gs[2], ptr(q), qs[0], qs[1], qs[2], ptr(k), ks[0], ks[1], ks[2],
+             ptr(v), vs[0], vs[1], vs[2], ptr(o), os_[0], os_[1], os_[2], ptr(lse), B, Tq, Tk, Hq, Hk, D, *how, ptr(dq), ptr(dk),
+             ptr(dv), ptr(work), floats)
+    return dq, dk, dv

@@ -1,0 +1,324 @@
+"""Attention (ops.attention_fwd / _bwd, interactions.attention) against softmax and its derivative in 64 bits.
+
+Tolerances, per element, from the sizes of the terms (u = 2^-24, every fp32 step is off by u relative):
+  a score z is a sum of D products: off by dz = (D + 8) u scale |q|.|k| + 8 u (|z| + |lse| + 1), the second part for the
+  exponent's own arithmetic; a probability is off by 2 dz of itself;
+  a sum over n keys or rows accumulates n + 64 roundings at most;
+  16-bit types round p and ds to half a step for their second product (fp16 to no less than half of its smallest number),
+  and o before delta is formed from it;
+  a result is rounded once: half a step."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def half_step(t, ref):
+    return torch.finfo(t).eps / 2 * ref.abs() + torch.finfo(t).smallest_normal * torch.finfo(t).eps
+
+
+def inside(got, ref, tol, what):
+    assert got.shape == ref.shape, what
+    over = (got.double() - ref).abs() - tol
+    assert bool((over <= 0).all()), f"{what}: {over.max().item():.3g} over the tolerance (of {tol.flatten()[over.argmax()].item():.3g})"
+
+
+def visible(B, Tq, Tk, lengths, query_lengths, causal, query_start):
+    i, j = torch.arange(Tq, device="cuda").view(1, -1, 1), torch.arange(Tk, device="cuda").view(1, 1, -1)
+    see = torch.ones(B, Tq, Tk, dtype=torch.bool, device="cuda")
+    if lengths is not None:
+        see = see & (j < lengths.view(-1, 1, 1))
+    if query_lengths is not None:
+        see = see & (i < query_lengths.view(-1, 1, 1))
+    if causal:
+        start = Tk - Tq if query_start is None else query_start.view(-1, 1, 1) if isinstance(query_start, torch.Tensor) else query_start
+        see = see & (j <= i + start)
+    return see
+
+
+def reference(q, k, v, do=None, lengths=None, query_lengths=None, causal=False, query_start=None, scale=None):
+    """Values and tolerances by name."""
+    B, Tq, Hq, D = q.shape
+    Tk, Hk = k.shape[1], k.shape[2]
+    G, t = Hq // Hk, q.dtype
+    low = 0.0 if t == torch.float32 else torch.finfo(t).eps / 2
+    tiny = torch.finfo(t).smallest_normal * torch.finfo(t).eps / 2 if t == torch.float16 else 0.0
+    scale = D ** -0.5 if scale is None else scale
+    see = visible(B, Tq, Tk, lengths, query_lengths, causal, query_start)
+    key_live = see.any(1).view(B, Tk, 1, 1)
+    row_live = see.any(2).view(B, Tq, 1, 1)
+    zero = lambda x, live: torch.where(live, x.double(), 0.0)          # noqa: E731
+    hd = lambda x: x.transpose(1, 2)                                    # noqa: E731  [B, H, T, D]
+    qd, kd, vd = hd(zero(q, row_live)), hd(zero(k, key_live)).repeat_interleave(G, 1), hd(zero(v, key_live)).repeat_interleave(G, 1)
+    T = lambda x: x.transpose(-1, -2).contiguous()                      # noqa: E731
+    see = see.unsqueeze(1)
+    seen = see.double()
+    z = scale * (qd @ T(kd))
+    lse = torch.where(see, z, -torch.inf).logsumexp(-1, keepdim=True)
+    p = torch.where(see, torch.exp(z - torch.where(lse == -torch.inf, 0.0, lse)), 0.0)
+    fin = torch.where(lse == -torch.inf, 0.0, lse).abs()
+    dz = (D + 8) * U * scale * (qd.abs() @ T(kd.abs())) + 8 * U * (z.abs() + fin + 1)
+    o = p @ vd
+    perr = p * (2 * dz + (Tk + 64) * U + low)
+    otol = perr @ vd.abs() + tiny * seen @ vd.abs()
+    out = {"o": (hd(o), half_step(t, hd(o)) + hd(otol)),
+           "lse": (lse.squeeze(-1), (2 * torch.where(see, dz, 0.0).amax(-1) + (Tk + 64) * U + 4 * U * fin.squeeze(-1)))}
+    if do is None:
+        return out
+    g = hd(zero(do, row_live))
+    dp, delta = g @ T(vd), (g * o).sum(-1, keepdim=True)
+    ds = p * (dp - delta)
+    dperr = (D + 8) * U * (g.abs() @ T(vd.abs()))
+    delerr = (g.abs() * (otol + half_step(t, o) + D * U * o.abs())).sum(-1, keepdim=True)
+    dserr = p * (2 * dz + 8 * U) * (dp.abs() + delta.abs()) + p * (dperr + delerr) + low * ds.abs() + tiny
+    dserr = torch.where(see, dserr, 0.0)
+    dq, dqt = scale * (ds @ kd), scale * ((dserr + (Tk + 64) * U * ds.abs()) @ kd.abs())
+    rows = (Tq + 64) * U * G
+    dk, dkt = scale * (T(ds) @ qd), scale * (T(dserr + rows * ds.abs()) @ qd.abs())
+    dv, dvt = T(p) @ g, T(p * (2 * dz + 8 * U + low + rows) + tiny * seen) @ g.abs()
+    share = lambda x: hd(x.view(B, Hk, G, Tk, D).sum(2))                # noqa: E731
+    out["dq"] = (hd(dq), half_step(t, hd(dq)) + hd(dqt))
+    for n, x, e in (("dk", dk, dkt), ("dv", dv, dvt)):
+        out[n] = (share(x), half_step(t, share(x)) + share(e))
+    return out
+
+
+def compare(q, k, v, do, **how):
+    from recommendsystem_amd import ops
+    ref = reference(q, k, v, do, **how)
+    o, lse = ops.attention_fwd(q, k, v, **how)
+    assert o.is_contiguous()
+    inside(o, *ref["o"], "o")
+    empty = ref["lse"][0] == -torch.inf
+    assert torch.equal(lse == -torch.inf, empty)
+    inside(lse[~empty], ref["lse"][0][~empty], ref["lse"][1][~empty], "lse")
+    if do is not None:
+        for name, got in zip(("dq", "dk", "dv"), ops.attention_bwd(do, q, k, v, o, lse, **how)):
+            inside(got, *ref[name], name)
+
+
+def make(B, Tq, Tk, Hq, Hk, D, kind, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    rn = lambda *s: torch.randn(*s, device="cuda", generator=g).to(TYPES[kind])     # noqa: E731
+    return rn(B, Tq, Hq, D), rn(B, Tk, Hk, D), rn(B, Tk, Hk, D), rn(B, Tq, Hq, D)
+
+
+def some_lengths(B, T, seed):
+    n = torch.randint(0, T + 1, (B,), device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed), dtype=torch.int32)
+    n[0] = T
+    if B > 1:
+        n[1] = 0
+    return n
+
+
+# B, Tq, Tk, Hq, Hk, D: single keys and rows, ends inside a tile and at its edge, padded and odd head sizes, shared key heads
+SHAPES = [(1, 1, 1, 1, 1, 1), (5, 39, 39, 2, 2, 16), (3, 5, 7, 4, 2, 20), (2, 64, 64, 2, 1, 32), (2, 65, 65, 3, 3, 64),
+          (2, 130, 130, 4, 1, 128), (3, 33, 257, 2, 2, 80), (2, 300, 300, 6, 2, 96), (3, 1, 500, 8, 2, 128), (4, 1, 33, 4, 4, 40),
+          (2, 17, 200, 3, 1, 7), (3, 200, 17, 2, 1, 33), (2, 129, 129, 1, 1, 63), (1, 2, 2, 10, 2, 24), (2, 96, 640, 5, 1, 64)]
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("B,Tq,Tk,Hq,Hk,D", SHAPES)
+def test_shapes_types_and_masks(B, Tq, Tk, Hq, Hk, D, causal, ragged, kind):
+    q, k, v, do = make(B, Tq, Tk, Hq, Hk, D, kind, seed=Tq * 7 + Tk + D)
+    how = dict(causal=causal)
+    if ragged:
+        how["lengths"] = some_lengths(B, Tk, 1)
+        how["query_lengths"] = how["lengths"] if Tq == Tk else some_lengths(B, Tq, 2)
+    compare(q, k, v, do, **how)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("fill", [float("nan"), float("inf"), "lowest"])
+def test_what_lies_behind_the_lengths_is_never_used(kind, fill):
+    fill = torch.finfo(TYPES[kind]).min if fill == "lowest" else fill
+    B, Tq, Tk = 4, 70, 150
+    q, k, v, do = make(B, Tq, Tk, 4, 2, 48, kind, seed=3)
+    n, m = some_lengths(B, Tk, 4), some_lengths(B, Tq, 5)
+    m[1] = 40                                    # rows that have no key at all (n[1] = 0)
+    past_k = torch.arange(Tk, device="cuda") >= n.view(-1, 1)
+    past_q = torch.arange(Tq, device="cuda") >= m.view(-1, 1)
+    for causal in (False, True):
+        for t, past in ((q, past_q), (do, past_q), (k, past_k), (v, past_k)):
+            t.masked_fill_(past[:, :, None, None], fill)
+        compare(q, k, v, do, lengths=n, query_lengths=m, causal=causal)
+    # keys no row sees under the causal mask, and rows in front of the first key
+    q, k, v, do = make(2, 50, 90, 2, 1, 32, kind, seed=6)
+    k[:, 70:], v[:, 70:] = fill, fill
+    compare(q, k, v, do, causal=True, query_start=20)
+    q[:, :30], do[:, :30] = fill, fill
+    compare(q, k, v, do, causal=True, query_start=-30)
+
+
+def test_query_starts_and_lengths_out_of_range():
+    q, k, v, do = make(5, 20, 100, 4, 2, 64, "bf16", seed=7)
+    start = torch.tensor([0, 80, -5, 33, 1000], device="cuda", dtype=torch.int32)
+    compare(q, k, v, do, causal=True, query_start=start)
+    n = torch.tensor([100, 90, 100, 40, 13], device="cuda", dtype=torch.int32)
+    compare(q, k, v, do, causal=True, query_start=start, lengths=n)
+    from recommendsystem_amd import ops
+    wild = torch.tensor([-7, 2 ** 31 - 1, 100, -2 ** 31, 0], device="cuda", dtype=torch.int32)
+    tame = wild.clamp(0, 100)
+    a, b = (ops.attention_fwd(q, k, v, lengths=t, query_lengths=t.clamp(max=20) if t is tame else t) for t in (wild, tame))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    ga, gb = (ops.attention_bwd(do, q, k, v, *a, lengths=t, query_lengths=t.clamp(max=20) if t is tame else t) for t in (wild, tame))
+    assert all(torch.equal(x, y) for x, y in zip(ga, gb))
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+def test_scores_of_every_size(kind):
+    """Scores far apart (one key takes all), large common offsets and a scale of its own."""
+    q, k, v, do = make(2, 40, 70, 2, 1, 32, kind, seed=8)
+    compare(q * 6, k * 6, v, do)
+    compare(q, k, v, do, scale=1e-3)
+    k2 = k.clone()
+    k2[..., 0] = 8.0
+    q2 = q.clone()
+    q2[..., 0] = 16.0
+    compare(q2, k2, v, do, scale=1.0)
+    compare(-q2, k2, v, do, scale=0.5, causal=True)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_strides_and_orders(kind):
+    B, T, H, D = 2, 45, 6, 32
+    qkv = torch.randn(B, T, 3 * H, D, device="cuda").to(TYPES[kind])
+    do = torch.randn(B, T, H, D, device="cuda").to(TYPES[kind])
+    compare(qkv[:, :, :H], qkv[:, :, H:2 * H], qkv[:, :, 2 * H:], do)
+    heads_first = qkv.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3)
+    compare(heads_first[:, :, :H], heads_first[:, :, H:H + 2], heads_first[:, :, -2:], do.permute(2, 0, 1, 3).contiguous().permute(1, 2, 0, 3))
+    compare(qkv[..., 1:28][:, :, :H], qkv[..., 2:29][:, :, H:2 * H], qkv[..., 3:30][:, :, 2 * H:], do[..., :27], causal=True)     # unaligned
+    dims = qkv.transpose(2, 3)                                                            # last dimension not contiguous
+    compare(dims[..., :8][:, :, :4], dims[..., 8:16][:, :, :2], dims[..., 2:10][:, :, :2], do.transpose(2, 3)[:, :, :4, :6].repeat(1, 1, 1, 2)[..., :8])
+    compare(qkv[:1, :, :H].expand(B, T, H, D), qkv[:, :1, :H].expand(B, T, H, D), qkv[:, :, :1].expand(B, T, H, D), do[:, :1].expand(B, T, H, D))
+    compare(qkv.flip(1)[:, :, :H], qkv[:, ::3, H:2 * H], qkv[:, 1:44:3, 2 * H:], do)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("Tq,G,D", [(1, 1, 64), (1, 4, 128), (3, 8, 32), (7, 2, 100)])
+def test_few_rows_over_a_long_cache(kind, Tq, G, D):
+    """The keys of a sample are split between workgroups and the shares joined."""
+    from recommendsystem_amd import _lib
+    B, Tk, Hk = 3, 5003, 2
+    assert _lib.lib().rs_attention_fwd_workspace_floats(0, B, Tq, Tk, G * Hk, Hk, D) > 0
+    q, k, v, _ = make(B, Tq, Tk, G * Hk, Hk, D, kind, seed=Tq)
+    n = torch.tensor([5003, 0, 1234], device="cuda", dtype=torch.int32)
+    compare(q, k, v, None, lengths=n)
+    compare(q, k, v, None, causal=True)
+    k[2, 1234:], v[2, 1234:], k[1], v[1] = float("nan"), float("nan"), float("inf"), float("nan")
+    compare(q, k, v, None, lengths=n, causal=True, query_start=n - Tq)
+
+
+def test_offsets_past_32_bits():
+    B, T, H, D = 2, 40, 2, 64
+    far = (1 << 31) + 4096
+    store = torch.empty(far + T * 3 * H * D, device="cuda", dtype=torch.bfloat16)
+    qkv = store.as_strided((B, T, 3 * H, D), (far, 3 * H * D, D, 1))
+    qkv.copy_(torch.randn(B, T, 3 * H, D, device="cuda"))
+    do = torch.randn(B, T, H, D, device="cuda").bfloat16()
+    compare(qkv[:, :, :H], qkv[:, :, H:2 * H], qkv[:, :, 2 * H:], do, causal=True)
+    compare(qkv[:, :1, :H], qkv[:, :, H:2 * H], qkv[:, :, 2 * H:], None)
+
+
+def test_autograd_and_differences():
+    from recommendsystem_amd import interactions as X
+    torch.manual_seed(11)
+    q = torch.randn(2, 9, 4, 16, device="cuda", requires_grad=True)
+    k = torch.randn(1, 12, 2, 16, device="cuda", requires_grad=True)
+    v = torch.randn(2, 12, 2, 16, device="cuda", requires_grad=True)
+    g = torch.randn(2, 9, 4, 16, device="cuda")
+    n = torch.tensor([12, 5], device="cuda", dtype=torch.int32)
+    f = lambda q, k, v: (X.attention(q, k.expand(2, -1, -1, -1), v, lengths=n, causal=True) * g).double().sum()      # noqa: E731
+    grads = torch.autograd.grad(f(q, k, v), (q, k, v))
+    ref = reference(q.detach(), k.detach().expand(2, -1, -1, -1), v.detach(), g, lengths=n, causal=True)
+    inside(grads[0], *ref["dq"], "dq")
+    inside(grads[1], ref["dk"][0].sum(0, keepdim=True), ref["dk"][1].sum(0, keepdim=True) + U * ref["dk"][0].abs().sum(0, keepdim=True), "dk")
+    inside(grads[2], *ref["dv"], "dv")
+    h = 2.0 ** -8
+    for i, t in enumerate((q, k, v)):
+        w = torch.randn_like(t)
+        w /= w.norm()
+        a = [x.detach() for x in (q, k, v)]
+        up, down = list(a), list(a)
+        up[i], down[i] = a[i] + h * w, a[i] - h * w
+        diff = (f(*up) - f(*down)) / (2 * h)
+        # 1152 terms of size below 4, each off by under 64 roundings, over 2h, adding up like their root; h^2 of curvature
+        assert abs(float(diff - (grads[i].double() * w).sum())) <= 1152 ** 0.5 * 4 * 64 * U / h + 20 * h * h
+    only = torch.autograd.grad(f(q.detach(), k.detach(), v), v)[0]
+    assert torch.equal(only, grads[2])
+
+
+def test_same_bits_on_two_streams_and_in_replayed_graphs():
+    from recommendsystem_amd import ops
+    q, k, v, do = make(3, 150, 150, 4, 2, 64, "bf16", seed=12)
+    n = some_lengths(3, 150, 13)
+    t, ck, cv, _ = make(2, 1, 3000, 8, 2, 64, "bf16", seed=14)
+
+    def step():
+        o, lse = ops.attention_fwd(q, k, v, lengths=n, query_lengths=n, causal=True)
+        return o, lse, *ops.attention_bwd(do, q, k, v, o, lse, lengths=n, query_lengths=n, causal=True), ops.attention_fwd(t, ck, cv)[0]
+
+    first = [x.clone() for x in step()]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+    outs = []
+    for _ in range(4):
+        for st in streams:
+            with torch.cuda.stream(st):
+                outs.append(step())
+    torch.cuda.synchronize()
+    for o in outs:
+        assert all(torch.equal(a, b) for a, b in zip(o, first))
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step()
+        graphs.append((g, out))
+    for seed in (1, 2, 3):
+        gen = torch.Generator(device="cuda").manual_seed(seed)
+        for x in (q, ck):
+            x.copy_(torch.randn(x.shape, device="cuda", generator=gen))
+        n.copy_(torch.randint(0, 151, (3,), device="cuda", generator=gen))
+        for st, (g, _) in zip(streams, graphs):              # both at once
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        want = step()
+        for _, out in graphs:
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_empty_and_refused():
+    from recommendsystem_amd import ops
+    from recommendsystem_amd._lib import RSError
+    q, k, v, do = make(2, 3, 5, 4, 2, 16, "f32", seed=15)
+    o, lse = ops.attention_fwd(q, k[:, :0], v[:, :0])        # no keys
+    assert torch.count_nonzero(o).item() == 0 and bool((lse == -torch.inf).all())
+    dq, dk, dv = ops.attention_bwd(do, q, k[:, :0], v[:, :0], o, lse)
+    assert torch.count_nonzero(dq).item() == 0 and dk.shape == (2, 0, 2, 16)
+    o, lse = ops.attention_fwd(q[:, :0], k, v)               # no rows
+    dq, dk, dv = ops.attention_bwd(do[:, :0], q[:, :0], k, v, o, lse)
+    assert o.shape == (2, 0, 4, 16) and torch.count_nonzero(dk).item() == 0 and torch.count_nonzero(dv).item() == 0
+    assert ops.attention_fwd(q[:0], k[:0], v[:0])[0].shape == (0, 3, 4, 16)
+    n = torch.tensor([3, 5], device="cuda", dtype=torch.int32)
+    big = torch.randn(2, 3, 2, 129, device="cuda")
+    bad = [lambda: ops.attention_fwd(q.double(), k.double(), v.double()), lambda: ops.attention_fwd(q, k.half(), v.half()),
+           lambda: ops.attention_fwd(q[0], k, v), lambda: ops.attention_fwd(q, k, v[:, :4]), lambda: ops.attention_fwd(q[:1], k, v),
+           lambda: ops.attention_fwd(q[:, :, :3], k, v), lambda: ops.attention_fwd(q[..., :8], k, v), lambda: ops.attention_fwd(big, big, big),
+           lambda: ops.attention_fwd(q, k[:, :, :0], v[:, :, :0]), lambda: ops.attention_fwd(q, k, v, lengths=n.long()),
+           lambda: ops.attention_fwd(q, k, v, lengths=n[:1]), lambda: ops.attention_fwd(q, k, v, query_lengths=n.cpu()),
+           lambda: ops.attention_fwd(q, k, v, query_start=n[:1]), lambda: ops.attention_fwd(q, k, v, query_start=2 ** 31),
+           lambda: ops.attention_fwd(q, k, v, scale=0.0), lambda: ops.attention_fwd(q, k, v, scale=float("nan")),
+           lambda: ops.attention_fwd(q.cpu(), k.cpu(), v.cpu()), lambda: ops.attention_fwd(q, k.cpu(), v),
+           lambda: ops.attention_bwd(do, q, k, v, q, torch.zeros(2, 3, 4, device="cuda")), lambda: ops.attention_bwd(do[:, :2], q, k, v, q, lse)]
+    for f in bad:
+        with pytest.raises(RSError):
+            f()

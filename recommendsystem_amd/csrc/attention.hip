@@ -49,7 +49,7 @@ struct AttnArgs {
     int tiles, splits;                       // row (key) tiles per (sample, key head); shares of the keys
     long long units;                         // workgroups with work
     float *part_o, *part_ml;                 // with splits > 1: [splits, B * Hk, Tq * G, D], lse in base 2 [.., Tq * G]
-    int vec;                                 // 16-byte accesses to q, k, v, o, go
+    int vec;                                 // 16-byte loads from q, k, v, o, go
     int out_vec;                             // four elements at once to the outputs
 };
 
@@ -81,46 +81,55 @@ template <> struct Mma<_Float16> {
     }
 };
 
-// A tile of R rows in LDS, DP elements and 16 bytes of padding to a row: consecutive rows start 4 banks apart.
+// A tile of rows in LDS, DP elements to a row in units of 16 bytes, unit u of row r in place u ^ swz(r): 16 rows at one unit
+// (the direct fragment) and 8 rows by four neighbouring units (the transposed one) both spread over all 64 banks, and a
+// row keeps its place in memory order, which is what the loads into LDS need.
 template <typename T, int DP> struct Tile {
-    static constexpr int RS = DP + 16 / (int)sizeof(T);
+    static constexpr int E = Mma<T>::E, UPR = DP / E;
     typedef typename Mma<T>::V V;
-
-    // rows row0 + lane % 32, elements of contraction step c
+    static __device__ __forceinline__ int swz(int r) {
+        if constexpr (UPR >= 16) return ((r & 3) << 2) | ((r >> 2) & 3);
+        else if constexpr (UPR == 8) return ((r & 2) << 1) | ((r >> 2) & 3);
+        else return (r >> 2) & 3;
+    }
+    // rows row0 + lane % 32 (row0 a multiple of 32), elements of contraction step c
     static __device__ __forceinline__ V rows(const T* lds, int row0, int c) {
-        const int l = threadIdx.x & 63;
-        return *(const V*)(lds + (row0 + (l & 31)) * RS + c * Mma<T>::CK + (l >> 5) * Mma<T>::E);
+        const int l = threadIdx.x & 63, r = l & 31;
+        return *(const V*)(lds + (row0 + r) * DP + (((2 * c + (l >> 5)) ^ swz(r)) * E));
     }
     // transposed: element col0 + lane % 32 of the rows that the registers of a product hold for contraction step c --
-    // half h of the wave has rows 4h .. 4h+3 of each group of eight
+    // half h of the wave has rows 4h .. 4h+3 of each group of eight; row0 is a multiple of CK
     static __device__ __forceinline__ V cols(const T* lds, int row0, int col0) {
         const int l = threadIdx.x & 63;
         if constexpr (sizeof(T) == 4) {
-            V r;
-            const T* p = lds + (row0 + 4 * (l >> 5)) * RS + col0 + (l & 31);
+            V v;
+            const int col = col0 + (l & 31);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) r[i] = p[i * RS];
-            return r;
+            for (int i = 0; i < 4; ++i) {
+                const int r = row0 + 4 * (l >> 5) + i;
+                v[i] = lds[r * DP + ((col / E) ^ swz(r)) * E + col % E];
+            }
+            return v;
         } else {
             // 16 lanes read 4 rows of 16 elements and get one element of each row
-            const T* p = lds + (row0 + 4 * (l >> 5) + ((l & 15) >> 2)) * RS + col0 + 16 * ((l >> 4) & 1) + 4 * (l & 3);
+            const int r = row0 + 4 * (l >> 5) + ((l & 15) >> 2), col = col0 + 16 * ((l >> 4) & 1) + 4 * (l & 3);
             typedef __attribute__((address_space(3))) rs_s16x4* lds_ptr;
-            union { rs_s16x4 s[2]; V v; } r;
-            r.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)p);
-            r.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 8 * RS));
-            return r.v;
+            union { rs_s16x4 s[2]; V v; } f;
+            f.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(lds + r * DP + ((col / E) ^ swz(r)) * E + col % E));
+            f.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(lds + (r + 8) * DP + ((col / E) ^ swz(r + 8)) * E + col % E));
+            return f.v;
         }
     }
 };
 
 // E elements from column col of a row of D (zeros behind D, and everywhere when the row has no part).
-template <typename T> __device__ __forceinline__ typename Mma<T>::V fetch(const T* row, int col, int D, int vec, bool live) {
+template <typename T, bool VEC> __device__ __forceinline__ typename Mma<T>::V fetch(const T* row, int col, int D, bool live) {
     typename Mma<T>::V r;
     constexpr int E = Mma<T>::E;
 #pragma unroll
     for (int e = 0; e < E; ++e) r[e] = (T)0.f;
     if (live && col < D) {
-        if (vec) {
+        if constexpr (VEC) {
             r = *(const typename Mma<T>::V*)(row + col);
         } else {
 #pragma unroll
@@ -131,26 +140,64 @@ template <typename T> __device__ __forceinline__ typename Mma<T>::V fetch(const 
     return r;
 }
 
-// A tile's way from memory through registers into LDS: NT lanes, R rows.
-template <typename T, int DP, int R, int NT> struct Stage {
-    static constexpr int E = Mma<T>::E, PER_ROW = DP / E, N = R * PER_ROW / NT;
-    static_assert(R * PER_ROW % NT == 0, "the lanes share a tile evenly");
-    typename Mma<T>::V r[N];
-    __device__ __forceinline__ void load(const T* base, long long row_stride, int row0, int row_end, int D, int vec) {
+// A tile's way into LDS: NT lanes, R rows; rows from row_end on and columns from D on become zeros.
+// VEC: asynchronous 16-byte loads from memory to LDS through a buffer descriptor that ends with the last row, whose range
+// check supplies the zeros; no register holds the data, and the tile is there after the wait in feed_sync().
+// Else (rows that do not start at multiples of 16 bytes): element by element through registers, land() writes them to LDS.
+template <typename T, int DP, int R, int NT, bool VEC> struct Feed {
+    typedef Tile<T, DP> L;
+    typedef typename Mma<T>::V V;
+    static constexpr int E = Mma<T>::E, UPR = L::UPR, N = R * UPR / NT;
+    static_assert(R * UPR % NT == 0, "the lanes share a tile evenly");
+    unsigned off[VEC ? N : 1];
+    V reg[VEC ? 1 : N];
+
+    __device__ __forceinline__ void init(long long stride, int D) {
+        if constexpr (VEC) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int x = threadIdx.x + i * NT, row = row0 + x / PER_ROW;
-            r[i] = fetch<T>(base + row * row_stride, (x % PER_ROW) * E, D, vec, row < row_end);
+            for (int i = 0; i < N; ++i) {
+                const int x = threadIdx.x + i * NT, r = x / UPR, u = (x % UPR) ^ L::swz(r);
+                off[i] = u * E < D ? (unsigned)(r * stride * sizeof(T) + u * 16) : 0x7ffffff0u;
+            }
         }
     }
-    __device__ __forceinline__ void store(T* lds) const {
+    // base: row 0; everything but off is the same in all lanes
+    __device__ __forceinline__ void begin(const T* base, long long stride, int row0, int row_end, int D, T* lds) {
+        if constexpr (VEC) {
+            const unsigned long long at = (unsigned long long)(base + row0 * stride);
+            long long bytes = ((row_end - row0 - 1) * stride + D) * (long long)sizeof(T);
+            bytes = bytes < 0x7fffff00LL ? bytes : 0x7fffff00LL;
+            typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+            const u32x4 rsrc = {(unsigned)__builtin_amdgcn_readfirstlane((int)at),
+                                (unsigned)__builtin_amdgcn_readfirstlane((int)(at >> 32)) & 0xffffu,
+                                (unsigned)__builtin_amdgcn_readfirstlane((int)bytes), 0x00027000u};
+            const unsigned dst = __builtin_amdgcn_readfirstlane(
+                (int)(unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)lds + (int)(threadIdx.x >> 6) * 1024);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int x = threadIdx.x + i * NT;
-            *(typename Mma<T>::V*)(lds + (x / PER_ROW) * Tile<T, DP>::RS + (x % PER_ROW) * E) = r[i];
+            for (int i = 0; i < N; ++i)      // the nops: a descriptor register written by a vector instruction just before
+                asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst + i * NT * 16),
+                             "v"(off[i]), "s"(rsrc)
+                             : "memory");
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int x = threadIdx.x + i * NT, r = x / UPR, u = (x % UPR) ^ L::swz(r);
+                reg[i] = fetch<T, false>(base + (row0 + r) * stride, u * E, D, row0 + r < row_end);
+            }
+        }
+    }
+    __device__ __forceinline__ void land(T* lds) const {
+        if constexpr (!VEC) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) *(V*)(lds + (threadIdx.x + i * NT) * E) = reg[i];
         }
     }
 };
+// This wave's loads have arrived and its reads are done, then everybody's.
+template <bool VEC> __device__ __forceinline__ void feed_sync() {
+    if constexpr (VEC) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    else __syncthreads();
+}
 
 // The registers of contraction step c of a product as the next product's B operand.
 template <typename T> __device__ __forceinline__ typename Mma<T>::V pack(const rs_f32x16& s, int c) {
@@ -206,13 +253,13 @@ template <typename T> __device__ __forceinline__ void store4(T* row, int d, int 
 template <typename T, int DP> constexpr int tile_rows() { return sizeof(T) == 4 && DP == 128 ? 32 : 64; }
 
 // ---- forward -----------------------------------------------------------------------------------------------------
-template <typename T, int DP, int NW, int KT>
+template <typename T, int DP, int NW, int KT, bool VEC>
 __global__ __launch_bounds__(NW * 64) void attention_fwd_kernel(const AttnArgs a) {
     constexpr int NT = NW * 64, BM = NW * 32, CK = Mma<T>::CK, E = Mma<T>::E, NC = DP / CK, NB = DP / 32, KB = KT / 32;
     typedef typename Mma<T>::V V;
     typedef Tile<T, DP> L;
-    __shared__ __align__(16) T s_k[2][KT * L::RS];
-    __shared__ __align__(16) T s_v[2][KT * L::RS];
+    __shared__ __align__(1024) T s_k[2][KT * DP];
+    __shared__ __align__(1024) T s_v[2][KT * DP];
     const long long unit = unit_of(rs_block_id(), a.units);
     if (unit >= a.units) return;
     const int split = (int)(unit % a.splits);
@@ -246,7 +293,7 @@ __global__ __launch_bounds__(NW * 64) void attention_fwd_kernel(const AttnArgs a
     {
         const T* qr = row_ptr<T>(a.q, b, live ? i : 0, live ? h : 0);
 #pragma unroll
-        for (int c = 0; c < NC; ++c) qf[c] = fetch<T>(qr, c * CK + half * E, a.D, a.vec, live && lim > 0);
+        for (int c = 0; c < NC; ++c) qf[c] = fetch<T, VEC>(qr, c * CK + half * E, a.D, live && lim > 0);
     }
     rs_f32x16 acc[NB];
 #pragma unroll
@@ -257,18 +304,20 @@ __global__ __launch_bounds__(NW * 64) void attention_fwd_kernel(const AttnArgs a
     const float scale2 = a.scale * LOG2E;
     const T* kp = row_ptr<T>(a.k, b, 0, hk);
     const T* vp = row_ptr<T>(a.v, b, 0, hk);
-    Stage<T, DP, KT, NT> sk, sv;
+    Feed<T, DP, KT, NT, VEC> fk, fv;
+    fk.init(a.k.t, a.D);
+    fv.init(a.v.t, a.D);
     if (k0 < end) {
-        sk.load(kp, a.k.t, k0, end, a.D, a.vec);
-        sv.load(vp, a.v.t, k0, end, a.D, a.vec);
+        fk.begin(kp, a.k.t, k0, end, a.D, s_k[0]);
+        fv.begin(vp, a.v.t, k0, end, a.D, s_v[0]);
     }
     for (int buf = 0; k0 < end; k0 += KT, buf ^= 1) {
-        sk.store(s_k[buf]);
-        sv.store(s_v[buf]);
-        __syncthreads();       // the other buffer's readers are past it: they stored this one after their last read
+        fk.land(s_k[buf]);
+        fv.land(s_v[buf]);
+        feed_sync<VEC>();      // the other buffer's readers are past it, too
         if (k0 + KT < end) {
-            sk.load(kp, a.k.t, k0 + KT, end, a.D, a.vec);
-            sv.load(vp, a.v.t, k0 + KT, end, a.D, a.vec);
+            fk.begin(kp, a.k.t, k0 + KT, end, a.D, s_k[buf ^ 1]);
+            fv.begin(vp, a.v.t, k0 + KT, end, a.D, s_v[buf ^ 1]);
         }
         rs_f32x16 s[KB];
 #pragma unroll
@@ -293,7 +342,7 @@ __global__ __launch_bounds__(NW * 64) void attention_fwd_kernel(const AttnArgs a
         top = fmaxf(top, other_half(top)) * scale2;
         const float m_new = fmaxf(m, top);
         const float base = m_new == -INFINITY ? 0.f : m_new;     // nothing seen yet: exp2(-inf - 0) = 0 throughout
-        const float alpha = exp2f(m - base);
+        const float alpha = __builtin_amdgcn_exp2f(m - base);
         m = m_new;
         float sum = 0.f;
 #pragma unroll
@@ -378,14 +427,14 @@ template <typename T> __global__ __launch_bounds__(256) void attention_join_kern
 }
 
 // ---- dq, and delta for the other gradients -----------------------------------------------------------------------------
-template <typename T, int DP, int NW>
+template <typename T, int DP, int NW, bool VEC>
 __global__ __launch_bounds__(NW * 64) void attention_dq_kernel(const AttnArgs a) {
     constexpr int KT = tile_rows<T, DP>();
     constexpr int NT = NW * 64, BM = NW * 32, CK = Mma<T>::CK, E = Mma<T>::E, NC = DP / CK, NB = DP / 32, KB = KT / 32;
     typedef typename Mma<T>::V V;
     typedef Tile<T, DP> L;
-    __shared__ __align__(16) T s_k[2][KT * L::RS];
-    __shared__ __align__(16) T s_v[2][KT * L::RS];
+    __shared__ __align__(1024) T s_k[2][KT * DP];
+    __shared__ __align__(1024) T s_v[2][KT * DP];
     const long long unit = unit_of(rs_block_id(), a.units);
     if (unit >= a.units) return;
     const int tile = a.tiles - 1 - (int)(unit % a.tiles);
@@ -415,9 +464,9 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_kernel(const AttnArgs a)
         const T* orow = row_ptr<T>(a.o, b, live ? i : 0, live ? h : 0);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            qf[c] = fetch<T>(qr, c * CK + half * E, a.D, a.vec, has);
-            gf[c] = fetch<T>(gr, c * CK + half * E, a.D, a.vec, has);
-            const V of = fetch<T>(orow, c * CK + half * E, a.D, a.vec, has);
+            qf[c] = fetch<T, VEC>(qr, c * CK + half * E, a.D, has);
+            gf[c] = fetch<T, VEC>(gr, c * CK + half * E, a.D, has);
+            const V of = fetch<T, VEC>(orow, c * CK + half * E, a.D, has);
 #pragma unroll
             for (int e = 0; e < E; ++e) delta += (float)gf[c][e] * (float)of[e];
         }
@@ -434,18 +483,20 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_kernel(const AttnArgs a)
     const float scale2 = a.scale * LOG2E;
     const T* kp = row_ptr<T>(a.k, b, 0, hk);
     const T* vp = row_ptr<T>(a.v, b, 0, hk);
-    Stage<T, DP, KT, NT> sk, sv;
+    Feed<T, DP, KT, NT, VEC> fk, fv;
+    fk.init(a.k.t, a.D);
+    fv.init(a.v.t, a.D);
     if (0 < end) {
-        sk.load(kp, a.k.t, 0, end, a.D, a.vec);
-        sv.load(vp, a.v.t, 0, end, a.D, a.vec);
+        fk.begin(kp, a.k.t, 0, end, a.D, s_k[0]);
+        fv.begin(vp, a.v.t, 0, end, a.D, s_v[0]);
     }
     for (int k0 = 0, buf = 0; k0 < end; k0 += KT, buf ^= 1) {
-        sk.store(s_k[buf]);
-        sv.store(s_v[buf]);
-        __syncthreads();
+        fk.land(s_k[buf]);
+        fv.land(s_v[buf]);
+        feed_sync<VEC>();      // the other buffer's readers are past it, too
         if (k0 + KT < end) {
-            sk.load(kp, a.k.t, k0 + KT, end, a.D, a.vec);
-            sv.load(vp, a.v.t, k0 + KT, end, a.D, a.vec);
+            fk.begin(kp, a.k.t, k0 + KT, end, a.D, s_k[buf ^ 1]);
+            fv.begin(vp, a.v.t, k0 + KT, end, a.D, s_v[buf ^ 1]);
         }
 #pragma unroll
         for (int n = 0; n < KB; ++n) {
@@ -486,16 +537,15 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_kernel(const AttnArgs a)
 }
 
 // ---- dk and dv -----------------------------------------------------------------------------------------------------------
-template <typename T, int DP, int NW>
+template <typename T, int DP, int NW, bool VEC>
 __global__ __launch_bounds__(NW * 64) void attention_dkv_kernel(const AttnArgs a) {
     constexpr int RT = tile_rows<T, DP>();
     constexpr int NT = NW * 64, BN = NW * 32, CK = Mma<T>::CK, E = Mma<T>::E, NC = DP / CK, NB = DP / 32, RB = RT / 32;
     typedef typename Mma<T>::V V;
     typedef Tile<T, DP> L;
-    __shared__ __align__(16) T s_q[2][RT * L::RS];
-    __shared__ __align__(16) T s_g[2][RT * L::RS];
+    __shared__ __align__(1024) T s_q[2][RT * DP];
+    __shared__ __align__(1024) T s_g[2][RT * DP];
     __shared__ __align__(16) float s_lse[2][RT], s_delta[2][RT];
-    __shared__ __align__(16) int s_lim[2][RT];
     const long long unit = unit_of(rs_block_id(), a.units);
     if (unit >= a.units) return;
     const int tile = (int)(unit % a.tiles);                       // causal: the first keys are seen by the most rows
@@ -505,21 +555,24 @@ __global__ __launch_bounds__(NW * 64) void attention_dkv_kernel(const AttnArgs a
     const int len = a.len ? min(max(a.len[b], 0), a.Tk) : a.Tk;
     const int qrows = a.qlen ? min(max(a.qlen[b], 0), a.Tq) : a.Tq;
     int begin = 0;                                                // first row that sees a key of this workgroup
+    long long start = 0;
     if (a.causal) {
-        const long long f = (long long)tile * BN - (a.qstart ? a.qstart[b] : a.start);
+        start = a.qstart ? a.qstart[b] : a.start;
+        const long long f = (long long)tile * BN - start;
         begin = f <= 0 ? 0 : f >= qrows ? qrows : (int)f;
     }
     const int stop = tile * BN < len ? qrows : 0;
 
+    // a key that no row sees is none: zeros here and in the results, whatever it holds
+    const bool has = key < len && qrows > 0 && (!a.causal || key <= start + qrows - 1);
     V kf[NC], vf[NC];
     {
-        const bool has = key < len;
         const T* kr = row_ptr<T>(a.k, b, has ? key : 0, hk);
         const T* vr = row_ptr<T>(a.v, b, has ? key : 0, hk);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            kf[c] = fetch<T>(kr, c * CK + half * E, a.D, a.vec, has);
-            vf[c] = fetch<T>(vr, c * CK + half * E, a.D, a.vec, has);
+            kf[c] = fetch<T, VEC>(kr, c * CK + half * E, a.D, has);
+            vf[c] = fetch<T, VEC>(vr, c * CK + half * E, a.D, has);
         }
     }
     rs_f32x16 dk[NB], dv[NB];
@@ -528,34 +581,42 @@ __global__ __launch_bounds__(NW * 64) void attention_dkv_kernel(const AttnArgs a
 #pragma unroll
         for (int e = 0; e < 16; ++e) dk[n][e] = dv[n][e] = 0.f;
     const float scale2 = a.scale * LOG2E;
-    Stage<T, DP, RT, NT> sq, sg;
+    Feed<T, DP, RT, NT, VEC> fq, fg;
+    fq.init(a.q.t, a.D);
+    fg.init(a.go.t, a.D);
     float r_lse = INFINITY, r_delta = 0.f;
-    int r_lim = 0;
     const int per_head = begin < stop ? (stop - begin + RT - 1) / RT : 0, turns = per_head * a.G;
     // turn -> (head of the group, row tile)
-    auto load = [&](int turn) {
-        const int h = hk * a.G + turn / per_head, r0 = begin + turn % per_head * RT;
-        sq.load(row_ptr<T>(a.q, b, 0, h), a.q.t, r0, stop, a.D, a.vec);
-        sg.load(row_ptr<T>(a.go, b, 0, h), a.go.t, r0, stop, a.D, a.vec);
+    int g = 0, r0 = begin;
+    auto load = [&](int buf) {
+        const int h = hk * a.G + g;
+        fq.begin(row_ptr<T>(a.q, b, 0, h), a.q.t, r0, stop, a.D, s_q[buf]);
+        fg.begin(row_ptr<T>(a.go, b, 0, h), a.go.t, r0, stop, a.D, s_g[buf]);
         if (threadIdx.x < RT) {
             const int i = r0 + threadIdx.x;
-            r_lim = i < stop ? row_limit(a, b, i) : 0;
             const long long at = ((long long)b * a.Hk * a.G + h) * a.Tq + i;
-            r_lse = r_lim > 0 ? a.lse[at] * LOG2E : INFINITY;     // a row that sees nothing: exp2(-inf) = 0
-            r_delta = r_lim > 0 ? a.delta[at] : 0.f;
+            const float x = i < stop ? a.lse[at] * LOG2E : -INFINITY;
+            r_lse = x == -INFINITY ? INFINITY : x;                // a row that sees nothing, or is none: exp2(z - inf) = 0
+            r_delta = i < stop ? a.delta[at] : 0.f;
         }
     };
     if (turns > 0) load(0);
     for (int turn = 0, buf = 0; turn < turns; ++turn, buf ^= 1) {
-        sq.store(s_q[buf]);
-        sg.store(s_g[buf]);
+        // a key that row r0 + x does not see: x < hide (selected below, not multiplied: it may hold anything)
+        const long long ahead = (long long)key - start - r0;
+        const int hide = !a.causal || ahead <= 0 ? 0 : ahead < RT ? (int)ahead : RT;
+        fq.land(s_q[buf]);
+        fg.land(s_g[buf]);
         if (threadIdx.x < RT) {
             s_lse[buf][threadIdx.x] = r_lse;
             s_delta[buf][threadIdx.x] = r_delta;
-            s_lim[buf][threadIdx.x] = r_lim;
         }
-        __syncthreads();
-        if (turn + 1 < turns) load(turn + 1);
+        feed_sync<VEC>();
+        if ((r0 += RT) >= stop) {
+            r0 = begin;
+            ++g;
+        }
+        if (turn + 1 < turns) load(buf ^ 1);
 #pragma unroll
         for (int n = 0; n < RB; ++n) {
             rs_f32x16 s, dp;
@@ -570,15 +631,17 @@ __global__ __launch_bounds__(NW * 64) void attention_dkv_kernel(const AttnArgs a
             for (int e = 0; e < 16; e += 4) {
                 const int r = n * 32 + reg_row(e);
                 const rs_f32x4 ls = *(const rs_f32x4*)&s_lse[buf][r], de = *(const rs_f32x4*)&s_delta[buf][r];
-                const int4 li = *(const int4*)&s_lim[buf][r];
-                const int lim[4] = {li.x, li.y, li.z, li.w};
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
-                    const bool seen = key < lim[x];               // selected, not multiplied: an unseen key may hold anything
-                    const float p = seen ? __builtin_amdgcn_exp2f(s[e + x] * scale2 - ls[x]) : 0.f;
+                    const float p = __builtin_amdgcn_exp2f(s[e + x] * scale2 - ls[x]);
                     s[e + x] = p;
-                    dp[e + x] = seen ? p * (dp[e + x] - de[x]) : 0.f;
+                    dp[e + x] = p * (dp[e + x] - de[x]);
                 }
+            }
+            if (__any(hide > n * 32)) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (n * 32 + reg_row(e) < hide) s[e] = dp[e] = 0.f;
             }
 #pragma unroll
             for (int c = 0; c < 32 / CK; ++c) {
@@ -600,8 +663,8 @@ __global__ __launch_bounds__(NW * 64) void attention_dkv_kernel(const AttnArgs a
             float o[4], u[4];
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-                o[x] = dk[d][e + x] * a.scale;
-                u[x] = dv[d][e + x];
+                o[x] = has ? dk[d][e + x] * a.scale : 0.f;
+                u[x] = has ? dv[d][e + x] : 0.f;
             }
             store4<T>((T*)a.dk + at, d * 32 + reg_row(e), a.D, a.out_vec, o);
             store4<T>((T*)a.dv + at, d * 32 + reg_row(e), a.D, a.out_vec, u);
@@ -627,7 +690,8 @@ int splits_for(int dtype, int B, int Tq, int Tk, int Hk, int G, int D) {
 template <typename T, int DP, int NW> int launch_fwd(const AttnArgs& a, hipStream_t stream) {
     constexpr int KT = NW == 1 ? 32 : tile_rows<T, DP>();
     const dim3 grid = rs_grid((a.units + 7) / 8 * 8);
-    hipLaunchKernelGGL((attention_fwd_kernel<T, DP, NW, KT>), grid, dim3(NW * 64), 0, stream, a);
+    if (a.vec) hipLaunchKernelGGL((attention_fwd_kernel<T, DP, NW, KT, true>), grid, dim3(NW * 64), 0, stream, a);
+    else hipLaunchKernelGGL((attention_fwd_kernel<T, DP, NW, KT, false>), grid, dim3(NW * 64), 0, stream, a);
     RS_CHECK_LAUNCH("rs_attention_fwd");
     if (a.splits > 1) {
         hipLaunchKernelGGL((attention_join_kernel<T>), rs_grid(rs_cdiv((long long)a.B * a.Hk * a.Tq * a.G, 4)), dim3(256), 0, stream, a);
@@ -646,14 +710,18 @@ template <typename T> int launch_fwd(const AttnArgs& a, int nw, hipStream_t stre
 template <typename T, int DP, int NW> int launch_dq(AttnArgs a, hipStream_t stream) {
     a.tiles = rs_cdiv((long long)a.Tq * a.G, NW * 32);
     a.units = (long long)a.B * a.Hk * a.tiles;
-    hipLaunchKernelGGL((attention_dq_kernel<T, DP, NW>), rs_grid((a.units + 7) / 8 * 8), dim3(NW * 64), 0, stream, a);
+    const dim3 grid = rs_grid((a.units + 7) / 8 * 8);
+    if (a.vec) hipLaunchKernelGGL((attention_dq_kernel<T, DP, NW, true>), grid, dim3(NW * 64), 0, stream, a);
+    else hipLaunchKernelGGL((attention_dq_kernel<T, DP, NW, false>), grid, dim3(NW * 64), 0, stream, a);
     RS_CHECK_LAUNCH("rs_attention_bwd");
     return RS_OK;
 }
 template <typename T, int DP, int NW> int launch_dkv(AttnArgs a, hipStream_t stream) {
     a.tiles = rs_cdiv(a.Tk, NW * 32);
     a.units = (long long)a.B * a.Hk * a.tiles;
-    hipLaunchKernelGGL((attention_dkv_kernel<T, DP, NW>), rs_grid((a.units + 7) / 8 * 8), dim3(NW * 64), 0, stream, a);
+    const dim3 grid = rs_grid((a.units + 7) / 8 * 8);
+    if (a.vec) hipLaunchKernelGGL((attention_dkv_kernel<T, DP, NW, true>), grid, dim3(NW * 64), 0, stream, a);
+    else hipLaunchKernelGGL((attention_dkv_kernel<T, DP, NW, false>), grid, dim3(NW * 64), 0, stream, a);
     RS_CHECK_LAUNCH("rs_attention_bwd");
     return RS_OK;
 }
@@ -689,9 +757,11 @@ bool shape_ok(const char* who, int dtype, int B, int Tq, int Tk, int Hq, int Hk,
     return true;
 }
 
-bool operand_vec(const Operand& x, int dtype) {
+// 16-byte loads through a descriptor that ends with the last row: rows start at multiples of 16 bytes, do not overlap (T rows
+// of one sample; a single row has no stride), and a tile of them stays within 31 bits.
+bool operand_vec(const Operand& x, int dtype, int T, int D) {
     const int e = 16 / rs_elem_bytes(dtype);
-    return !x.p || (rs_aligned16(x.p) && x.b % e == 0 && x.t % e == 0 && x.h % e == 0);
+    return !x.p || (rs_aligned16(x.p) && x.b % e == 0 && x.h % e == 0 && (T <= 1 || (x.t % e == 0 && x.t >= D)) && x.t < (1 << 23));
 }
 
 }  // namespace
@@ -722,7 +792,7 @@ int rs_attention_fwd(int dtype, const void* q, long long qb, long long qt, long 
     a.qstart = query_starts;
     a.B = B, a.Tq = Tq, a.Tk = Tk, a.Hk = Hk, a.G = Hq / Hk, a.D = D, a.causal = causal != 0, a.start = query_start;
     a.scale = scale;
-    a.vec = D % (16 / rs_elem_bytes(dtype)) == 0 && operand_vec(a.q, dtype) && operand_vec(a.k, dtype) && operand_vec(a.v, dtype);
+    a.vec = D % (16 / rs_elem_bytes(dtype)) == 0 && operand_vec(a.q, dtype, Tq, D) && operand_vec(a.k, dtype, Tk, D) && operand_vec(a.v, dtype, Tk, D);
     a.out_vec = D % 4 == 0 && rs_aligned16(o);
     const long long rows = (long long)Tq * a.G;
     const int nw = waves_for(rows);
@@ -774,8 +844,8 @@ int rs_attention_bwd(int dtype, const void* go, long long gb, long long gt, long
     a.B = B, a.Tq = Tq, a.Tk = Tk, a.Hk = Hk, a.G = Hq / Hk, a.D = D, a.causal = causal != 0, a.start = query_start;
     a.scale = scale;
     a.splits = 1;
-    a.vec = D % (16 / rs_elem_bytes(dtype)) == 0 && operand_vec(a.q, dtype) && operand_vec(a.k, dtype) && operand_vec(a.v, dtype) &&
-            operand_vec(a.o, dtype) && operand_vec(a.go, dtype);
+    a.vec = D % (16 / rs_elem_bytes(dtype)) == 0 && operand_vec(a.q, dtype, Tq, D) && operand_vec(a.k, dtype, Tk, D) && operand_vec(a.v, dtype, Tk, D) &&
+            operand_vec(a.o, dtype, Tq, D) && operand_vec(a.go, dtype, Tq, D);
     a.out_vec = D % 4 == 0 && rs_aligned16(dq) && rs_aligned16(dk) && rs_aligned16(dv);
     if (dtype == RS_F32) return launch_bwd<float>(a, stream);
     if (dtype == RS_BF16) return launch_bwd<__bf16>(a, stream);

@@ -140,7 +140,7 @@ template <typename T, bool VEC> __device__ __forceinline__ typename Mma<T>::V fe
     return r;
 }
 
-// A tile's way into LDS: NT lanes, R rows; rows from row_end on and columns from D on become zeros.
+// The way of consecutive tiles of R rows into LDS, NT lanes; rows from row_end on and columns from D on become zeros.
 // VEC: asynchronous 16-byte loads from memory to LDS through a buffer descriptor that ends with the last row, whose range
 // check supplies the zeros; no register holds the data, and the tile is there after the wait in feed_sync().
 // Else (rows that do not start at multiples of 16 bytes): element by element through registers, land() writes them to LDS.
@@ -151,8 +151,11 @@ template <typename T, int DP, int R, int NT, bool VEC> struct Feed {
     static_assert(R * UPR % NT == 0, "the lanes share a tile evenly");
     unsigned off[VEC ? N : 1];
     V reg[VEC ? 1 : N];
+    const T* at;                 // first row of the next tile
+    long long stride, left;      // left: elements from there to the end of the last row
+    int rows, D;
 
-    __device__ __forceinline__ void init(long long stride, int D) {
+    __device__ __forceinline__ Feed(long long row_stride, int d) : stride(row_stride), D(d) {
         if constexpr (VEC) {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
@@ -161,16 +164,21 @@ template <typename T, int DP, int R, int NT, bool VEC> struct Feed {
             }
         }
     }
-    // base: row 0; everything but off is the same in all lanes
-    __device__ __forceinline__ void begin(const T* base, long long stride, int row0, int row_end, int D, T* lds) {
+    // the next tile is row0's (the same in all lanes)
+    __device__ __forceinline__ void seek(const T* base, int row0, int row_end) {
+        at = base + row0 * stride;
+        rows = row_end - row0;
+        left = (rows - 1) * stride + D;
+    }
+    __device__ __forceinline__ void next(T* lds) {
         if constexpr (VEC) {
-            const unsigned long long at = (unsigned long long)(base + row0 * stride);
-            long long bytes = ((row_end - row0 - 1) * stride + D) * (long long)sizeof(T);
-            bytes = bytes < 0x7fffff00LL ? bytes : 0x7fffff00LL;
+            const unsigned long long where = (unsigned long long)at;
+            const long long most = 0x7fffff00LL / (int)sizeof(T);
+            const int bytes = (int)(left < most ? left : most) * (int)sizeof(T);
             typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-            const u32x4 rsrc = {(unsigned)__builtin_amdgcn_readfirstlane((int)at),
-                                (unsigned)__builtin_amdgcn_readfirstlane((int)(at >> 32)) & 0xffffu,
-                                (unsigned)__builtin_amdgcn_readfirstlane((int)bytes), 0x00027000u};
+            const u32x4 rsrc = {(unsigned)__builtin_amdgcn_readfirstlane((int)where),
+                                (unsigned)__builtin_amdgcn_readfirstlane((int)(where >> 32)) & 0xffffu,
+                                (unsigned)__builtin_amdgcn_readfirstlane(bytes), 0x00027000u};
             const unsigned dst = __builtin_amdgcn_readfirstlane(
                 (int)(unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)lds + (int)(threadIdx.x >> 6) * 1024);
 #pragma unroll
@@ -182,9 +190,12 @@ template <typename T, int DP, int R, int NT, bool VEC> struct Feed {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const int x = threadIdx.x + i * NT, r = x / UPR, u = (x % UPR) ^ L::swz(r);
-                reg[i] = fetch<T, false>(base + (row0 + r) * stride, u * E, D, row0 + r < row_end);
+                reg[i] = fetch<T, false>(at + r * stride, u * E, D, r < rows);
             }
         }
+        at += R * stride;
+        rows -= R;
+        left -= R * stride;
     }
     __device__ __forceinline__ void land(T* lds) const {
         if constexpr (!VEC) {
@@ -193,6 +204,15 @@ template <typename T, int DP, int R, int NT, bool VEC> struct Feed {
         }
     }
 };
+// A fragment that was loaded in front of a loop has arrived: without a use there, the wait for it would stand in the loop
+// and hold up the asynchronous loads, too.
+template <typename V> __device__ __forceinline__ void settle(V& v) {
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    union { V v; u32x4 u; } x;
+    x.v = v;
+    asm volatile("" : "+v"(x.u));
+    v = x.v;
+}
 // This wave's loads have arrived and its reads are done, then everybody's.
 template <bool VEC> __device__ __forceinline__ void feed_sync() {
     if constexpr (VEC) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -304,20 +324,22 @@ __global__ __launch_bounds__(NW * 64) void attention_fwd_kernel(const AttnArgs a
     const float scale2 = a.scale * LOG2E;
     const T* kp = row_ptr<T>(a.k, b, 0, hk);
     const T* vp = row_ptr<T>(a.v, b, 0, hk);
-    Feed<T, DP, KT, NT, VEC> fk, fv;
-    fk.init(a.k.t, a.D);
-    fv.init(a.v.t, a.D);
+    Feed<T, DP, KT, NT, VEC> fk(a.k.t, a.D), fv(a.v.t, a.D);
+    fk.seek(kp, k0, end);
+    fv.seek(vp, k0, end);
     if (k0 < end) {
-        fk.begin(kp, a.k.t, k0, end, a.D, s_k[0]);
-        fv.begin(vp, a.v.t, k0, end, a.D, s_v[0]);
+        fk.next(s_k[0]);
+        fv.next(s_v[0]);
     }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) settle(qf[c]);
     for (int buf = 0; k0 < end; k0 += KT, buf ^= 1) {
         fk.land(s_k[buf]);
         fv.land(s_v[buf]);
         feed_sync<VEC>();      // the other buffer's readers are past it, too
         if (k0 + KT < end) {
-            fk.begin(kp, a.k.t, k0 + KT, end, a.D, s_k[buf ^ 1]);
-            fv.begin(vp, a.v.t, k0 + KT, end, a.D, s_v[buf ^ 1]);
+            fk.next(s_k[buf ^ 1]);
+            fv.next(s_v[buf ^ 1]);
         }
         rs_f32x16 s[KB];
 #pragma unroll
@@ -483,20 +505,25 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_kernel(const AttnArgs a)
     const float scale2 = a.scale * LOG2E;
     const T* kp = row_ptr<T>(a.k, b, 0, hk);
     const T* vp = row_ptr<T>(a.v, b, 0, hk);
-    Feed<T, DP, KT, NT, VEC> fk, fv;
-    fk.init(a.k.t, a.D);
-    fv.init(a.v.t, a.D);
+    Feed<T, DP, KT, NT, VEC> fk(a.k.t, a.D), fv(a.v.t, a.D);
+    fk.seek(kp, 0, end);
+    fv.seek(vp, 0, end);
     if (0 < end) {
-        fk.begin(kp, a.k.t, 0, end, a.D, s_k[0]);
-        fv.begin(vp, a.v.t, 0, end, a.D, s_v[0]);
+        fk.next(s_k[0]);
+        fv.next(s_v[0]);
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        settle(qf[c]);
+        settle(gf[c]);
     }
     for (int k0 = 0, buf = 0; k0 < end; k0 += KT, buf ^= 1) {
         fk.land(s_k[buf]);
         fv.land(s_v[buf]);
         feed_sync<VEC>();      // the other buffer's readers are past it, too
         if (k0 + KT < end) {
-            fk.begin(kp, a.k.t, k0 + KT, end, a.D, s_k[buf ^ 1]);
-            fv.begin(vp, a.v.t, k0 + KT, end, a.D, s_v[buf ^ 1]);
+            fk.next(s_k[buf ^ 1]);
+            fv.next(s_v[buf ^ 1]);
         }
 #pragma unroll
         for (int n = 0; n < KB; ++n) {
@@ -538,13 +565,15 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_kernel(const AttnArgs a)
 
 // ---- dk and dv -----------------------------------------------------------------------------------------------------------
 template <typename T, int DP, int NW, bool VEC>
-__global__ __launch_bounds__(NW * 64) void attention_dkv_kernel(const AttnArgs a) {
-    constexpr int RT = tile_rows<T, DP>();
+__global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 2 && VEC && NW == 4 ? 2 : 1) void attention_dkv_kernel(const AttnArgs a) {
+    constexpr bool VLDS = DP == 128 && sizeof(T) == 2;
+    constexpr int RT = VLDS ? 32 : tile_rows<T, DP>();
     constexpr int NT = NW * 64, BN = NW * 32, CK = Mma<T>::CK, E = Mma<T>::E, NC = DP / CK, NB = DP / 32, RB = RT / 32;
     typedef typename Mma<T>::V V;
     typedef Tile<T, DP> L;
     __shared__ __align__(1024) T s_q[2][RT * DP];
     __shared__ __align__(1024) T s_g[2][RT * DP];
+    __shared__ __align__(1024) T s_v[VLDS ? BN * DP : 1];
     __shared__ __align__(16) float s_lse[2][RT], s_delta[2][RT];
     const long long unit = unit_of(rs_block_id(), a.units);
     if (unit >= a.units) return;
@@ -565,14 +594,24 @@ __global__ __launch_bounds__(NW * 64) void attention_dkv_kernel(const AttnArgs a
 
     // a key that no row sees is none: zeros here and in the results, whatever it holds
     const bool has = key < len && qrows > 0 && (!a.causal || key <= start + qrows - 1);
-    V kf[NC], vf[NC];
+    V kf[NC], vf[VLDS ? 1 : NC];
     {
         const T* kr = row_ptr<T>(a.k, b, has ? key : 0, hk);
         const T* vr = row_ptr<T>(a.v, b, has ? key : 0, hk);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             kf[c] = fetch<T, VEC>(kr, c * CK + half * E, a.D, has);
-            vf[c] = fetch<T, VEC>(vr, c * CK + half * E, a.D, has);
+            if constexpr (!VLDS) vf[c] = fetch<T, VEC>(vr, c * CK + half * E, a.D, has);
+        }
+    }
+    if constexpr (VLDS) {
+        Feed<T, DP, BN, NT, VEC> fv(a.v.t, a.D);
+        const long long seen = a.causal ? start + qrows : len;     // keys below it are seen
+        const int end = qrows > 0 ? (int)max(0LL, min(seen, (long long)len)) : 0;
+        if (tile * BN < end) {
+            fv.seek(row_ptr<T>(a.v, b, 0, hk), tile * BN, end);
+            fv.next(s_v);
+            fv.land(s_v);
         }
     }
     rs_f32x16 dk[NB], dv[NB];
@@ -581,25 +620,32 @@ __global__ __launch_bounds__(NW * 64) void attention_dkv_kernel(const AttnArgs a
 #pragma unroll
         for (int e = 0; e < 16; ++e) dk[n][e] = dv[n][e] = 0.f;
     const float scale2 = a.scale * LOG2E;
-    Feed<T, DP, RT, NT, VEC> fq, fg;
-    fq.init(a.q.t, a.D);
-    fg.init(a.go.t, a.D);
-    float r_lse = INFINITY, r_delta = 0.f;
+    Feed<T, DP, RT, NT, VEC> fq(a.q.t, a.D), fg(a.go.t, a.D);
     const int per_head = begin < stop ? (stop - begin + RT - 1) / RT : 0, turns = per_head * a.G;
-    // turn -> (head of the group, row tile)
-    int g = 0, r0 = begin;
+    // a turn is a row tile of one head of the group; the loads run one turn ahead
+    int h = hk * a.G, r0 = begin, r_next = begin;
+    float r_lse, r_delta;
     auto load = [&](int buf) {
-        const int h = hk * a.G + g;
-        fq.begin(row_ptr<T>(a.q, b, 0, h), a.q.t, r0, stop, a.D, s_q[buf]);
-        fg.begin(row_ptr<T>(a.go, b, 0, h), a.go.t, r0, stop, a.D, s_g[buf]);
-        if (threadIdx.x < RT) {
-            const int i = r0 + threadIdx.x;
-            const long long at = ((long long)b * a.Hk * a.G + h) * a.Tq + i;
-            const float x = i < stop ? a.lse[at] * LOG2E : -INFINITY;
-            r_lse = x == -INFINITY ? INFINITY : x;                // a row that sees nothing, or is none: exp2(z - inf) = 0
-            r_delta = i < stop ? a.delta[at] : 0.f;
+        // all lanes, a valid row each, and used only when the tile has landed: a wait for these would wait for the tile
+        const long long at = ((long long)b * a.Hk * a.G + h) * a.Tq + min(r_next + (int)(threadIdx.x % RT), stop - 1);
+        r_lse = a.lse[at];
+        r_delta = a.delta[at];
+        if (r_next == begin) {
+            fq.seek(row_ptr<T>(a.q, b, 0, h), begin, stop);
+            fg.seek(row_ptr<T>(a.go, b, 0, h), begin, stop);
+        }
+        fq.next(s_q[buf]);
+        fg.next(s_g[buf]);
+        if ((r_next += RT) >= stop) {
+            r_next = begin;
+            ++h;
         }
     };
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        settle(kf[c]);
+        if constexpr (!VLDS) settle(vf[c]);
+    }
     if (turns > 0) load(0);
     for (int turn = 0, buf = 0; turn < turns; ++turn, buf ^= 1) {
         // a key that row r0 + x does not see: x < hide (selected below, not multiplied: it may hold anything)
@@ -607,15 +653,14 @@ __global__ __launch_bounds__(NW * 64) void attention_dkv_kernel(const AttnArgs a
         const int hide = !a.causal || ahead <= 0 ? 0 : ahead < RT ? (int)ahead : RT;
         fq.land(s_q[buf]);
         fg.land(s_g[buf]);
+        // a row that sees nothing, or is none: exp2(z - inf) = 0
+        asm volatile("" : "+v"(r_lse), "+v"(r_delta));            // all lanes wait for them here (see settle)
         if (threadIdx.x < RT) {
-            s_lse[buf][threadIdx.x] = r_lse;
+            s_lse[buf][threadIdx.x] = r_lse == -INFINITY || r0 + (int)threadIdx.x >= stop ? INFINITY : r_lse * LOG2E;
             s_delta[buf][threadIdx.x] = r_delta;
         }
         feed_sync<VEC>();
-        if ((r0 += RT) >= stop) {
-            r0 = begin;
-            ++g;
-        }
+        r0 = r_next;
         if (turn + 1 < turns) load(buf ^ 1);
 #pragma unroll
         for (int n = 0; n < RB; ++n) {
@@ -625,7 +670,10 @@ __global__ __launch_bounds__(NW * 64) void attention_dkv_kernel(const AttnArgs a
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 s = Mma<T>::mul(L::rows(s_q[buf], n * 32, c), kf[c], s);
-                dp = Mma<T>::mul(L::rows(s_g[buf], n * 32, c), vf[c], dp);
+                V vc;
+                if constexpr (VLDS) vc = L::rows(s_v, wave * 32, c);
+                else vc = vf[c];
+                dp = Mma<T>::mul(L::rows(s_g[buf], n * 32, c), vc, dp);
             }
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {

@@ -46,9 +46,10 @@ struct AttnArgs {
     const int *len, *qlen, *qstart;          // [B] or null
     int B, Tq, Tk, Hk, G, D, causal, start;
     float scale;
-    int tiles, splits;                       // row (key) tiles per (sample, key head); shares of the keys
-    long long units;                         // workgroups with work
-    float *part_o, *part_ml;                 // with splits > 1: [splits, B * Hk, Tq * G, D], lse in base 2 [.., Tq * G]
+    int tiles, splits;                       // row (key) tiles per (sample, key head); shares of the keys (rows)
+    int dealt;                               // order of the workgroups, see unit_of
+    // with splits > 1: forward [splits, B * Hk, Tq * G, D] and lse in base 2 [.., Tq * G], dk / dv [splits, 2, B, Tk, Hk, D]
+    float *part_o, *part_ml;
     int vec;                                 // 16-byte loads from q, k, v, o, go
     int out_vec;                             // four elements at once to the outputs
 };
@@ -231,11 +232,32 @@ __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 
 // Row of register i within a 32x32 result.
 __device__ __forceinline__ int reg_row(int i) { return 8 * (i >> 2) + 4 * ((threadIdx.x & 63) >> 5) + (i & 3); }
 
-// Workgroup -> unit of work: ids go round the eight XCDs, so that neighbouring units, which read the same keys, get to
-// one XCD and its L2.
-__device__ __forceinline__ long long unit_of(long long id, long long units) {
-    const long long per = (units + 7) / 8;
-    return (id >> 3) < per ? (id & 7) * per + (id >> 3) : units;
+// Workgroup -> (sample, key head) pair, tile and share; pair < 0: no work.  Workgroups go round the eight XCDs: all work on
+// one pair, which reads the same keys, gets to one XCD and its L2.  Many pairs are dealt out one by one, which spreads the
+// heads of a long sample over the XCDs; few are cut into eight runs of tiles, so that no XCD gets a pair more than another.
+struct Unit {
+    int pair, tile, split;
+};
+__device__ __forceinline__ Unit unit_of(const AttnArgs& a) {
+    const unsigned id = (unsigned)rs_block_id(), x = id & 7, j = id >> 3, splits = a.splits, per_pair = a.tiles * splits;
+    const unsigned pairs = (unsigned)a.B * a.Hk;
+    unsigned pair, in;
+    if (a.dealt) {
+        const unsigned k = j / per_pair;
+        pair = k * 8 + x;
+        in = j - k * per_pair;
+    } else {
+        const unsigned run = (pairs * per_pair + 7) / 8, unit = x * run + j;
+        pair = j < run ? unit / per_pair : pairs;
+        in = unit % per_pair;
+    }
+    if (pair >= pairs) return {-1, 0, 0};
+    return {(int)pair, (int)(in / splits), (int)(in % splits)};
+}
+inline long long order_units(AttnArgs& a) {      // the workgroups to launch for a.tiles and a.splits
+    const long long pairs = (long long)a.B * a.Hk, per_pair = (long long)a.tiles * a.splits;
+    a.dealt = pairs % 8 == 0 || pairs >= 64;
+    return a.dealt ? (pairs + 7) / 8 * 8 * per_pair : (pairs * per_pair + 7) / 8 * 8;
 }
 
 // What a lane's row sees: keys below the result.
@@ -280,15 +302,13 @@ __global__ __launch_bounds__(NW * 64) void attention_fwd_kernel(const AttnArgs a
     typedef Tile<T, DP> L;
     __shared__ __align__(1024) T s_k[2][KT * DP];
     __shared__ __align__(1024) T s_v[2][KT * DP];
-    const long long unit = unit_of(rs_block_id(), a.units);
-    if (unit >= a.units) return;
-    const int split = (int)(unit % a.splits);
-    const long long rest = unit / a.splits;
-    const int tile = a.tiles - 1 - (int)(rest % a.tiles);        // causal: the long rows first
-    const int pair = (int)(rest / a.tiles), b = pair / a.Hk, hk = pair % a.Hk;
+    const Unit unit = unit_of(a);
+    if (unit.pair < 0) return;
+    const int tile = a.tiles - 1 - unit.tile, split = unit.split;          // causal: the long rows first
+    const int pair = unit.pair, b = pair / a.Hk, hk = pair % a.Hk;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int rows = a.Tq * a.G, row = tile * BM + wave * 32 + (lane & 31);
-    const int i = row / a.G, h = hk * a.G + row % a.G;
+    const int i = (unsigned)row / (unsigned)a.G, h = hk * a.G + (unsigned)row % (unsigned)a.G;
     const bool live = row < rows;
     const int lim = live ? row_limit(a, b, i) : 0;
     // keys any row of the workgroup sees, and all live rows of this wave (rows only see more further down)
@@ -457,13 +477,13 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_kernel(const AttnArgs a)
     typedef Tile<T, DP> L;
     __shared__ __align__(1024) T s_k[2][KT * DP];
     __shared__ __align__(1024) T s_v[2][KT * DP];
-    const long long unit = unit_of(rs_block_id(), a.units);
-    if (unit >= a.units) return;
-    const int tile = a.tiles - 1 - (int)(unit % a.tiles);
-    const int pair = (int)(unit / a.tiles), b = pair / a.Hk, hk = pair % a.Hk;
+    const Unit unit = unit_of(a);
+    if (unit.pair < 0) return;
+    const int tile = a.tiles - 1 - unit.tile;
+    const int pair = unit.pair, b = pair / a.Hk, hk = pair % a.Hk;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int rows = a.Tq * a.G, row = tile * BM + wave * 32 + (lane & 31);
-    const int i = row / a.G, h = hk * a.G + row % a.G;
+    const int i = (unsigned)row / (unsigned)a.G, h = hk * a.G + (unsigned)row % (unsigned)a.G;
     const bool live = row < rows;
     const int lim = live ? row_limit(a, b, i) : 0;
     const int last = min(tile * BM + BM, rows) - 1;
@@ -575,10 +595,10 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 2 && VEC && NW =
     __shared__ __align__(1024) T s_g[2][RT * DP];
     __shared__ __align__(1024) T s_v[VLDS ? BN * DP : 1];
     __shared__ __align__(16) float s_lse[2][RT], s_delta[2][RT];
-    const long long unit = unit_of(rs_block_id(), a.units);
-    if (unit >= a.units) return;
-    const int tile = (int)(unit % a.tiles);                       // causal: the first keys are seen by the most rows
-    const int pair = (int)(unit / a.tiles), b = pair / a.Hk, hk = pair % a.Hk;
+    const Unit unit = unit_of(a);
+    if (unit.pair < 0) return;
+    const int tile = unit.tile, split = unit.split;               // causal: the first keys are seen by the most rows
+    const int pair = unit.pair, b = pair / a.Hk, hk = pair % a.Hk;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int key = tile * BN + wave * 32 + (lane & 31);
     const int len = a.len ? min(max(a.len[b], 0), a.Tk) : a.Tk;
@@ -621,24 +641,29 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 2 && VEC && NW =
         for (int e = 0; e < 16; ++e) dk[n][e] = dv[n][e] = 0.f;
     const float scale2 = a.scale * LOG2E;
     Feed<T, DP, RT, NT, VEC> fq(a.q.t, a.D), fg(a.go.t, a.D);
-    const int per_head = begin < stop ? (stop - begin + RT - 1) / RT : 0, turns = per_head * a.G;
-    // a turn is a row tile of one head of the group; the loads run one turn ahead
-    int h = hk * a.G, r0 = begin, r_next = begin;
+    // a turn is a row tile of one head of the group; this workgroup takes its share of them, the loads run one ahead
+    const int per_head = begin < stop ? (stop - begin + RT - 1) / RT : 0, all = per_head * a.G;
+    const int share = (all + a.splits - 1) / a.splits, turn0 = min(split * share, all), turns = min(turn0 + share, all) - turn0;
+    int h = hk * a.G, r_next = begin;
+    if (turns > 0) {
+        h += turn0 / per_head;
+        r_next += turn0 % per_head * RT;
+        fq.seek(row_ptr<T>(a.q, b, 0, h), r_next, stop);
+        fg.seek(row_ptr<T>(a.go, b, 0, h), r_next, stop);
+    }
+    int r0 = r_next;
     float r_lse, r_delta;
     auto load = [&](int buf) {
         // all lanes, a valid row each, and used only when the tile has landed: a wait for these would wait for the tile
         const long long at = ((long long)b * a.Hk * a.G + h) * a.Tq + min(r_next + (int)(threadIdx.x % RT), stop - 1);
         r_lse = a.lse[at];
         r_delta = a.delta[at];
-        if (r_next == begin) {
-            fq.seek(row_ptr<T>(a.q, b, 0, h), begin, stop);
-            fg.seek(row_ptr<T>(a.go, b, 0, h), begin, stop);
-        }
         fq.next(s_q[buf]);
         fg.next(s_g[buf]);
-        if ((r_next += RT) >= stop) {
+        if ((r_next += RT) >= stop && ++h < (hk + 1) * a.G) {
             r_next = begin;
-            ++h;
+            fq.seek(row_ptr<T>(a.q, b, 0, h), begin, stop);
+            fg.seek(row_ptr<T>(a.go, b, 0, h), begin, stop);
         }
     };
 #pragma unroll
@@ -714,9 +739,36 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 2 && VEC && NW =
                 o[x] = has ? dk[d][e + x] * a.scale : 0.f;
                 u[x] = has ? dv[d][e + x] : 0.f;
             }
-            store4<T>((T*)a.dk + at, d * 32 + reg_row(e), a.D, a.out_vec, o);
-            store4<T>((T*)a.dv + at, d * 32 + reg_row(e), a.D, a.out_vec, u);
+            if (a.splits > 1) {
+                const long long total = (long long)a.B * a.Tk * a.Hk * a.D;
+                store4<float>(a.part_o + 2 * split * total + at, d * 32 + reg_row(e), a.D, a.D % 4 == 0, o);
+                store4<float>(a.part_o + (2 * split + 1) * total + at, d * 32 + reg_row(e), a.D, a.D % 4 == 0, u);
+            } else {
+                store4<T>((T*)a.dk + at, d * 32 + reg_row(e), a.D, a.out_vec, o);
+                store4<T>((T*)a.dv + at, d * 32 + reg_row(e), a.D, a.out_vec, u);
+            }
         }
+}
+
+// dk and dv from the shares, added in their order.
+template <typename T> __global__ __launch_bounds__(256) void attention_dkv_join_kernel(const AttnArgs a) {
+    const long long total = (long long)a.B * a.Tk * a.Hk * a.D, at = (rs_block_id() * 256 + threadIdx.x) * 4;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        T* out = (T*)(w ? a.dv : a.dk);
+        if (at + 4 <= total && a.out_vec) {
+            rs_f32x4 x = *(const rs_f32x4*)(a.part_o + w * total + at);
+            for (int s = 1; s < a.splits; ++s) x += *(const rs_f32x4*)(a.part_o + (2 * s + w) * total + at);
+            const float o[4] = {x[0], x[1], x[2], x[3]};
+            store4<T>(out + at, 0, 4, true, o);
+        } else {
+            for (long long i = at; i < at + 4 && i < total; ++i) {
+                float x = 0.f;
+                for (int s = 0; s < a.splits; ++s) x += a.part_o[(2 * s + w) * total + i];
+                out[i] = (T)x;
+            }
+        }
+    }
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
@@ -735,9 +787,19 @@ int splits_for(int dtype, int B, int Tq, int Tk, int Hk, int G, int D) {
     return s < 1 ? 1 : s > 64 ? 64 : (int)s;
 }
 
-template <typename T, int DP, int NW> int launch_fwd(const AttnArgs& a, hipStream_t stream) {
+// Shares of the rows for dk and dv.  Even work: split until there are two workgroups for every CU.  A causal mask or lengths
+// give the key tiles uneven work, and one workgroup per key tile leaves some CUs with twice the mean: split until there are
+// four (2 x 8192 causal, 4 key heads, 512 key tiles: 1.79 ms in one share, 1.34 in two; without the mask one share
+// of as many tiles takes 1.20 ms, four 1.34).  No share is shorter than eight row tiles.
+int dkv_splits(int B, int Tq, int Tk, int Hk, int G, int uneven) {
+    const long long units = (long long)B * Hk * rs_cdiv(Tk, Tk <= 64 ? 64 : 128), turns = (long long)G * rs_cdiv(Tq, 64);
+    const long long want = (uneven ? 1024 : 512) / units, most = turns / 8, s = want < most ? want : most;
+    return s < 1 ? 1 : s > 16 ? 16 : (int)s;
+}
+
+template <typename T, int DP, int NW> int launch_fwd(AttnArgs a, hipStream_t stream) {
     constexpr int KT = NW == 1 ? 32 : tile_rows<T, DP>();
-    const dim3 grid = rs_grid((a.units + 7) / 8 * 8);
+    const dim3 grid = rs_grid(order_units(a));
     if (a.vec) hipLaunchKernelGGL((attention_fwd_kernel<T, DP, NW, KT, true>), grid, dim3(NW * 64), 0, stream, a);
     else hipLaunchKernelGGL((attention_fwd_kernel<T, DP, NW, KT, false>), grid, dim3(NW * 64), 0, stream, a);
     RS_CHECK_LAUNCH("rs_attention_fwd");
@@ -757,8 +819,8 @@ template <typename T> int launch_fwd(const AttnArgs& a, int nw, hipStream_t stre
 
 template <typename T, int DP, int NW> int launch_dq(AttnArgs a, hipStream_t stream) {
     a.tiles = rs_cdiv((long long)a.Tq * a.G, NW * 32);
-    a.units = (long long)a.B * a.Hk * a.tiles;
-    const dim3 grid = rs_grid((a.units + 7) / 8 * 8);
+    a.splits = 1;                            // a row's keys are not shared out here
+    const dim3 grid = rs_grid(order_units(a));
     if (a.vec) hipLaunchKernelGGL((attention_dq_kernel<T, DP, NW, true>), grid, dim3(NW * 64), 0, stream, a);
     else hipLaunchKernelGGL((attention_dq_kernel<T, DP, NW, false>), grid, dim3(NW * 64), 0, stream, a);
     RS_CHECK_LAUNCH("rs_attention_bwd");
@@ -766,11 +828,15 @@ template <typename T, int DP, int NW> int launch_dq(AttnArgs a, hipStream_t stre
 }
 template <typename T, int DP, int NW> int launch_dkv(AttnArgs a, hipStream_t stream) {
     a.tiles = rs_cdiv(a.Tk, NW * 32);
-    a.units = (long long)a.B * a.Hk * a.tiles;
-    const dim3 grid = rs_grid((a.units + 7) / 8 * 8);
+    const dim3 grid = rs_grid(order_units(a));
     if (a.vec) hipLaunchKernelGGL((attention_dkv_kernel<T, DP, NW, true>), grid, dim3(NW * 64), 0, stream, a);
     else hipLaunchKernelGGL((attention_dkv_kernel<T, DP, NW, false>), grid, dim3(NW * 64), 0, stream, a);
     RS_CHECK_LAUNCH("rs_attention_bwd");
+    if (a.splits > 1) {
+        const long long quads = ((long long)a.B * a.Tk * a.Hk * a.D + 3) / 4;
+        hipLaunchKernelGGL((attention_dkv_join_kernel<T>), rs_grid((quads + 255) / 256), dim3(256), 0, stream, a);
+        RS_CHECK_LAUNCH("rs_attention_bwd");
+    }
     return RS_OK;
 }
 template <typename T, int DP> int launch_bwd(const AttnArgs& a, hipStream_t stream) {
@@ -846,7 +912,6 @@ int rs_attention_fwd(int dtype, const void* q, long long qb, long long qt, long 
     const int nw = waves_for(rows);
     a.tiles = rs_cdiv(rows, nw * 32);
     a.splits = Tk > 0 ? splits_for(dtype, B, Tq, Tk, Hk, a.G, D) : 1;
-    a.units = (long long)B * Hk * a.tiles * a.splits;
     if (a.splits > 1) {
         const size_t need = rs_attention_fwd_workspace_floats(dtype, B, Tq, Tk, Hq, Hk, D);
         if (!workspace || workspace_floats < need) {
@@ -862,7 +927,12 @@ int rs_attention_fwd(int dtype, const void* q, long long qb, long long qt, long 
     return launch_fwd<_Float16>(a, nw, stream);
 }
 
-size_t rs_attention_bwd_workspace_floats(int B, int Tq, int Hq) { return B > 0 && Tq > 0 && Hq > 0 ? (size_t)B * Tq * Hq : 0; }
+size_t rs_attention_bwd_workspace_floats(int B, int Tq, int Tk, int Hq, int Hk, int D, int uneven) {
+    if (B <= 0 || Tq <= 0 || Tk < 0 || Hk < 1 || Hq < Hk || Hq % Hk || D < 1 || D > 128) return 0;
+    const int s = Tk > 0 ? dkv_splits(B, Tq, Tk, Hk, Hq / Hk, uneven) : 1;
+    // delta, up to a multiple of four floats, then the shares of dk and dv
+    return ((size_t)B * Tq * Hq + 3) / 4 * 4 + (s > 1 ? (size_t)2 * s * B * Tk * Hk * D : 0);
+}
 
 int rs_attention_bwd(int dtype, const void* go, long long gb, long long gt, long long gh, const void* q, long long qb, long long qt,
                      long long qh, const void* k, long long kb, long long kt, long long kh, const void* v, long long vb,
@@ -873,10 +943,13 @@ int rs_attention_bwd(int dtype, const void* go, long long gb, long long gt, long
     if (!shape_ok("rs_attention_bwd", dtype, B, Tq, Tk, Hq, Hk, D, scale)) return RS_ERR_ARG;
     if (B == 0 || (Tq == 0 && Tk == 0)) return RS_OK;
     RS_CHECK_ARG((Tq == 0 || (go && q && o && lse && dq)) && (Tk == 0 || (k && v && dk && dv)), "rs_attention_bwd: null argument");
-    if (Tq > 0 && (!workspace || workspace_floats < rs_attention_bwd_workspace_floats(B, Tq, Hq))) {
-        rs_set_error("rs_attention_bwd: workspace of %zu floats, %zu needed", workspace_floats, rs_attention_bwd_workspace_floats(B, Tq, Hq));
+    const int uneven = causal != 0 || lengths || query_lengths;
+    const size_t need = rs_attention_bwd_workspace_floats(B, Tq, Tk, Hq, Hk, D, uneven);
+    if (need && (!workspace || workspace_floats < need)) {
+        rs_set_error("rs_attention_bwd: workspace of %zu floats, %zu needed", workspace_floats, need);
         return RS_ERR_WORKSPACE;
     }
+    RS_CHECK_ARG(rs_aligned16(workspace), "rs_attention_bwd: workspace must be aligned to 16 bytes");
     AttnArgs a = {};
     a.q = {q, qb, qt, qh};
     a.k = {k, kb, kt, kh};
@@ -891,7 +964,8 @@ int rs_attention_bwd(int dtype, const void* go, long long gb, long long gt, long
     a.qstart = query_starts;
     a.B = B, a.Tq = Tq, a.Tk = Tk, a.Hk = Hk, a.G = Hq / Hk, a.D = D, a.causal = causal != 0, a.start = query_start;
     a.scale = scale;
-    a.splits = 1;
+    a.splits = Tq > 0 && Tk > 0 ? dkv_splits(B, Tq, Tk, Hk, a.G, uneven) : 1;
+    a.part_o = workspace + ((size_t)B * Tq * Hq + 3) / 4 * 4;
     a.vec = D % (16 / rs_elem_bytes(dtype)) == 0 && operand_vec(a.q, dtype, Tq, D) && operand_vec(a.k, dtype, Tk, D) && operand_vec(a.v, dtype, Tk, D) &&
             operand_vec(a.o, dtype, Tq, D) && operand_vec(a.go, dtype, Tq, D);
     a.out_vec = D % 4 == 0 && rs_aligned16(dq) && rs_aligned16(dk) && rs_aligned16(dv);

@@ -2040,7 +2040,8 @@ def attention_bwd(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.T
     dq = torch.empty((B, Tq, Hq, D), dtype=q.dtype, device=dev)
     dk = torch.empty((B, Tk, Hk, D), dtype=q.dtype, device=dev)
     dv = torch.empty((B, Tk, Hk, D), dtype=q.dtype, device=dev)
-    floats = _lib.lib().rs_attention_bwd_workspace_floats(B, Tq, Hq)
+    floats = _lib.lib().rs_attention_bwd_workspace_floats(
+        B, Tq, Tk, Hq, Hk, D, int(bool(causal) or lengths is not None or query_lengths is not None))
     work = torch.empty(max(floats, 1), dtype=torch.float32, device=dev)
     gs, qs, ks, vs, os_ = do.stride(), q.stride(), k.stride(), v.stride(), o.stride()
     _call_on(dev, "rs_attention_bwd", code, ptr(do), gs[0], gs[1], gs[2], ptr(q), qs[0], qs[1], qs[2], ptr(k), ks[0], ks[1], ks[2],

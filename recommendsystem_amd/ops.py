@@ -6,6 +6,7 @@ on torch's current stream.
 """
 from __future__ import annotations
 
+import functools
 import math
 import os
 from typing import List, Optional
@@ -1780,49 +1781,49 @@ def _elem_code(t: torch.Tensor, name: str) -> int:
     return code
 
 
-def _same_device(*named):
-    """All tensors (None allowed) on one GPU; returns it."""
-    dev = None
-    for name, t in named:
-        if t is None:
-            continue
-        require_cuda(t)
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise RSError(f"{name}: is on {t.device}, the first operand on {dev}")
+def _same_device(first: torch.Tensor, *others):
+    """The GPU all tensors (None allowed among the others) are on."""
+    require_cuda(first)
+    dev = first.device
+    for t in others:
+        if t is not None and t.device != dev:
+            require_cuda(t)
+            raise RSError(f"operands are on different devices: {dev} and {t.device}")
     return dev
 
 
 def _call_on(dev, name: str, *args):
     """call() on the current stream of the operands' device, whichever device is current."""
     if dev.index == torch._C._cuda_getDevice():
-        call(name, *args, stream())
+        call(name, *args, torch._C._cuda_getCurrentRawStream(dev.index))
     else:
         with torch.cuda.device(dev):
-            call(name, *args, stream())
+            call(name, *args, torch._C._cuda_getCurrentRawStream(dev.index))
 
 
-def _norm_rows(t: torch.Tensor, name: str, like: torch.Tensor):
-    """t as [rows, N] with contiguous elements in a row (a copy only where its strides allow no such view), and the row
-    stride."""
+def _addr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _norm_rows(t: torch.Tensor, name: str, like: torch.Tensor, N: int):
+    """(t as rows of N contiguous elements, row stride): t itself or a view, a copy only where its strides allow none."""
     if t.dtype != like.dtype or t.shape != like.shape:
         raise RSError(f"{name}: expected {like.dtype} {tuple(like.shape)}, got {t.dtype} {tuple(t.shape)}")
-    N = t.shape[-1]
-    r = t.reshape(-1, N) if t.numel() else t.reshape(0, N)
+    if t.is_contiguous():
+        return t, N
+    r = t.reshape(-1, N)
     if (N > 1 and r.stride(1) != 1) or (r.shape[0] > 1 and r.stride(0) < N):
         r = r.contiguous()
     return r, (r.stride(0) if r.shape[0] > 1 else N)
 
 
-def _norm_param_code(x: torch.Tensor, weight, bias) -> int:
+def _norm_param_code(x: torch.Tensor, N: int, weight, bias) -> int:
     """Element code of the weight and the bias (x's type or float32; the same for both)."""
-    N = x.shape[-1]
     dtype = None
     for name, p in (("weight", weight), ("bias", bias)):
         if p is None:
             continue
-        if tuple(p.shape) != (N,) or not p.is_contiguous():
+        if p.dim() != 1 or p.shape[0] != N or not p.is_contiguous():
             raise RSError(f"layer_norm: {name} must be a contiguous vector of {N}, got {tuple(p.shape)}")
         if p.dtype not in (x.dtype, torch.float32) or (dtype is not None and p.dtype != dtype):
             raise RSError(f"layer_norm: weight and bias must both be {x.dtype} or both float32, got {name} {p.dtype}")
@@ -1836,22 +1837,21 @@ def layer_norm_fwd(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias:
     dimension.  x: [..., N], float32 / bfloat16 / float16; weight and bias: [N] of x's type or float32, each may be None.
     Returns (y, s, mean, rstd): y and s like x, mean and rstd float32 with one value per row for layer_norm_bwd."""
     code = _elem_code(x, "layer_norm")
-    if x.dim() == 0 or x.shape[-1] == 0:
+    N = x.shape[-1] if x.dim() else 0
+    if N == 0:
         raise RSError(f"layer_norm: nothing to normalise in shape {tuple(x.shape)}")
-    pcode = _norm_param_code(x, weight, bias)
-    dev = _same_device(("x", x), ("weight", weight), ("bias", bias), ("residual", residual))
-    N = x.shape[-1]
-    x2, ldx = _norm_rows(x, "x", x)
-    M = x2.shape[0]
+    pcode = _norm_param_code(x, N, weight, bias)
+    dev = _same_device(x, weight, bias, residual)
+    x2, ldx = _norm_rows(x, "x", x, N)
+    r2, ldr = (None, 0) if residual is None else _norm_rows(residual, "residual", x, N)
+    M = x.numel() // N
     if M > 0x7FFFFFFF or N > 0x3FFFFFFF:
         raise RSError(f"layer_norm: {M} rows of {N} are too many")
-    r2, ldr = (None, 0) if residual is None else _norm_rows(residual, "residual", x)
     y = torch.empty(x.shape, dtype=x.dtype, device=dev)
     s = x if residual is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
-    stats = torch.empty((2, M), dtype=torch.float32, device=dev)
-    mean, rstd = stats[0], stats[1]
-    _call_on(dev, "rs_layer_norm_fwd", code, pcode, ptr(x2), ldx, ptr(r2), ldr, M, N, ptr(weight), ptr(bias), float(eps), ptr(y),
-             None if residual is None else ptr(s), ptr(mean), ptr(rstd))
+    mean, rstd = torch.empty((2, M), dtype=torch.float32, device=dev).unbind(0)
+    _call_on(dev, "rs_layer_norm_fwd", code, pcode, x2.data_ptr(), ldx, _addr(r2), ldr, M, N, _addr(weight), _addr(bias), float(eps),
+             y.data_ptr(), None if residual is None else s.data_ptr(), mean.data_ptr(), rstd.data_ptr())
     return y, s, mean, rstd
 
 
@@ -1861,32 +1861,36 @@ def layer_norm_bwd(dy: torch.Tensor, s: torch.Tensor, mean: torch.Tensor, rstd: 
     is the gradient of x and of the residual alike; dw and db are [N] of the weight's type (param_dtype, default s's type,
     where there is no weight), None without want_params.  The row sums are added in a fixed order."""
     code = _elem_code(s, "layer_norm")
-    if s.dim() == 0 or s.shape[-1] == 0:
+    N = s.shape[-1] if s.dim() else 0
+    if N == 0:
         raise RSError(f"layer_norm: nothing to normalise in shape {tuple(s.shape)}")
-    dev = _same_device(("s", s), ("dy", dy), ("mean", mean), ("rstd", rstd), ("weight", weight), ("ds", ds))
-    N = s.shape[-1]
-    s2, lds = _norm_rows(s, "s", s)
-    d2, ldd = _norm_rows(dy, "dy", s)
-    q2, ldq = (None, 0) if ds is None else _norm_rows(ds, "ds", s)
-    M = s2.shape[0]
+    dev = _same_device(s, dy, mean, rstd, weight, ds)
+    s2, lds = _norm_rows(s, "s", s, N)
+    d2, ldd = _norm_rows(dy, "dy", s, N)
+    q2, ldq = (None, 0) if ds is None else _norm_rows(ds, "ds", s, N)
+    M = s.numel() // N
     _chk(mean, torch.float32, "mean", (M,))
     _chk(rstd, torch.float32, "rstd", (M,))
     pdt = weight.dtype if weight is not None else (param_dtype or s.dtype)
     if pdt not in (s.dtype, torch.float32):
         raise RSError(f"layer_norm: parameters must be {s.dtype} or float32, got {pdt}")
-    pcode = _norm_param_code(s, weight, None) if weight is not None else _ELEM_CODES[pdt]
+    pcode = _norm_param_code(s, N, weight, None) if weight is not None else _ELEM_CODES[pdt]
     dx = torch.empty(s.shape, dtype=s.dtype, device=dev)
     dw = db = work = None
     floats = 0
     if want_params:
-        dw = torch.empty(N, dtype=pdt, device=dev)
-        db = torch.empty(N, dtype=pdt, device=dev)
-        floats = _lib.lib().rs_layer_norm_bwd_workspace_floats(M, N)
+        dw, db = torch.empty((2, N), dtype=pdt, device=dev).unbind(0)
+        floats = _norm_floats(M, N)
         # per call: two captured graphs, or two streams, never share the partial sums
         work = torch.empty(max(floats, 1), dtype=torch.float32, device=dev)
-    _call_on(dev, "rs_layer_norm_bwd", code, pcode, ptr(d2), ldd, ptr(s2), lds, ptr(mean), ptr(rstd), ptr(weight), ptr(q2), ldq, M,
-             N, ptr(dx), ptr(dw), ptr(db), ptr(work), floats)
+    _call_on(dev, "rs_layer_norm_bwd", code, pcode, d2.data_ptr(), ldd, s2.data_ptr(), lds, mean.data_ptr(), rstd.data_ptr(),
+             _addr(weight), _addr(q2), ldq, M, N, dx.data_ptr(), _addr(dw), _addr(db), _addr(work), floats)
     return dx, dw, db
+
+
+@functools.lru_cache(maxsize=4096)
+def _norm_floats(M: int, N: int) -> int:
+    return _lib.lib().rs_layer_norm_bwd_workspace_floats(M, N)
 
 
 class RotaryTable:
@@ -1956,14 +1960,14 @@ def rotary(table: RotaryTable, positions: torch.Tensor, q: torch.Tensor, k: Opti
         raise RSError(f"rotary: positions must be int64 or int32 [{T}] or [{B}, {T}], got {positions.dtype} {tuple(positions.shape)}")
     if (Hq + Hk) * D > 1 << 24 or B * T > 0x7FFFFFFF:
         raise RSError(f"rotary: {B * T} tokens of {Hq + Hk} heads of {D} are too many")
-    dev = _same_device(("q", q), ("k", k), ("positions", positions), ("table", table.cos))
+    dev = _same_device(q, k, positions, table.cos)
     pb, pt = positions.stride() if positions.dim() == 2 else (0, positions.stride(0))
     qo = torch.empty((B, T, Hq, D), dtype=q.dtype, device=dev)
     ko = torch.empty((B, T, Hk, D), dtype=q.dtype, device=dev) if k is not None else None
     qs, ks = q.stride(), (k.stride() if k is not None else (0, 0, 0))
-    _call_on(dev, "rs_rotary", code, ptr(q), qs[0], qs[1], qs[2], Hq, ptr(k), ks[0], ks[1], ks[2], Hk, B, T, D, table.rotary_dim,
-             int(table.interleaved), ptr(positions), int(positions.dtype == torch.int64), pb, pt, ptr(table.cos), ptr(table.sin),
-             table.max_positions, int(inverse), ptr(qo), ptr(ko), ptr(table.err_flag))
+    _call_on(dev, "rs_rotary", code, q.data_ptr(), qs[0], qs[1], qs[2], Hq, _addr(k), ks[0], ks[1], ks[2], Hk, B, T, D,
+             table.rotary_dim, table.interleaved, positions.data_ptr(), positions.dtype == torch.int64, pb, pt, table.cos.data_ptr(),
+             table.sin.data_ptr(), table.max_positions, inverse, qo.data_ptr(), _addr(ko), table.err_flag.data_ptr())
     return qo if k is None else (qo, ko)
 
 
@@ -1994,12 +1998,12 @@ def _attention_args(q, k, v, lengths, query_lengths, causal, query_start, scale)
     scale = D ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale <= 1e30:
         raise RSError(f"attention: scale must be positive and finite, got {scale}")
-    dev = _same_device(("q", q), ("k", k), ("v", v), ("lengths", lengths), ("query_lengths", query_lengths), ("query_start", starts))
-    return code, q, k, v, (B, Tq, Tk, Hq, Hk, D), (ptr(lengths), ptr(query_lengths), int(bool(causal)), ptr(starts), start, scale), dev
+    dev = _same_device(q, k, v, lengths, query_lengths, starts)
+    return code, q, k, v, (B, Tq, Tk, Hq, Hk, D), (_addr(lengths), _addr(query_lengths), bool(causal), _addr(starts), start, scale), dev
 
 
 def _chk_vector(t: torch.Tensor, name: str, n: int):
-    if t.dtype != torch.int32 or tuple(t.shape) != (n,) or not t.is_contiguous():
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
         raise RSError(f"attention: {name} must be a contiguous int32 vector of {n}, got {t.dtype} {tuple(t.shape)}")
 
 
@@ -2017,13 +2021,18 @@ def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: Op
     code, q, k, v, (B, Tq, Tk, Hq, Hk, D), how, dev = _attention_args(q, k, v, lengths, query_lengths, causal, query_start, scale)
     o = torch.empty((B, Tq, Hq, D), dtype=q.dtype, device=dev)
     lse = torch.empty((B, Hq, Tq), dtype=torch.float32, device=dev) if want_lse else None
-    floats = _lib.lib().rs_attention_fwd_workspace_floats(code, B, Tq, Tk, Hq, Hk, D)
+    floats = _attention_floats(code, B, Tq, Tk, Hq, Hk, D)
     # per call: two captured graphs, or two streams, never share the partial results
     work = torch.empty(floats, dtype=torch.float32, device=dev) if floats else None
     qs, ks, vs = q.stride(), k.stride(), v.stride()
-    _call_on(dev, "rs_attention_fwd", code, ptr(q), qs[0], qs[1], qs[2], ptr(k), ks[0], ks[1], ks[2], ptr(v), vs[0], vs[1], vs[2],
-             B, Tq, Tk, Hq, Hk, D, *how, ptr(o), ptr(lse), ptr(work), floats)
+    _call_on(dev, "rs_attention_fwd", code, q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0],
+             vs[1], vs[2], B, Tq, Tk, Hq, Hk, D, *how, o.data_ptr(), _addr(lse), _addr(work), floats)
     return o, lse
+
+
+@functools.lru_cache(maxsize=4096)
+def _attention_floats(*sizes) -> int:
+    return _lib.lib().rs_attention_fwd_workspace_floats(*sizes)
 
 
 def attention_bwd(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor,
@@ -2036,7 +2045,7 @@ def attention_bwd(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.T
     do = _heads_view(do, "do", q.shape, q.dtype)
     o = _heads_view(o, "o", q.shape, q.dtype)
     _chk(lse, torch.float32, "lse", (B, Hq, Tq))
-    dev = _same_device(("q", q), ("do", do), ("o", o), ("lse", lse))
+    dev = _same_device(q, do, o, lse)
     dq = torch.empty((B, Tq, Hq, D), dtype=q.dtype, device=dev)
     dk = torch.empty((B, Tk, Hk, D), dtype=q.dtype, device=dev)
     dv = torch.empty((B, Tk, Hk, D), dtype=q.dtype, device=dev)
@@ -2044,7 +2053,7 @@ def attention_bwd(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.T
         B, Tq, Tk, Hq, Hk, D, int(bool(causal) or lengths is not None or query_lengths is not None))
     work = torch.empty(max(floats, 1), dtype=torch.float32, device=dev)
     gs, qs, ks, vs, os_ = do.stride(), q.stride(), k.stride(), v.stride(), o.stride()
-    _call_on(dev, "rs_attention_bwd", code, ptr(do), gs[0], gs[1], gs[2], ptr(q), qs[0], qs[1], qs[2], ptr(k), ks[0], ks[1], ks[2],
-             ptr(v), vs[0], vs[1], vs[2], ptr(o), os_[0], os_[1], os_[2], ptr(lse), B, Tq, Tk, Hq, Hk, D, *how, ptr(dq), ptr(dk),
-             ptr(dv), ptr(work), floats)
+    _call_on(dev, "rs_attention_bwd", code, do.data_ptr(), gs[0], gs[1], gs[2], q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0],
+             ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2], o.data_ptr(), os_[0], os_[1], os_[2], lse.data_ptr(), B, Tq, Tk, Hq, Hk,
+             D, *how, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), work.data_ptr(), floats)
     return dq, dk, dv

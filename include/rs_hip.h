@@ -624,7 +624,7 @@ int rs_rotary(int dtype, const void* q, long long qb, long long qt, long long qh
  * rs_attention_bwd_workspace_floats(..) floats, 16-byte aligned (uneven: 1 with a causal mask or lengths).  No atomics: results do not change from run to run.
  * Stands beside rs_afm_fwd / _bwd (model/AFM/AFM.py:36-56), which pools field pairs with one softmax per sample. */
 size_t rs_attention_fwd_workspace_floats(int dtype, int B, int Tq, int Tk, int Hq, int Hk, int D);
-size_t rs_attention_bwd_workspace_floats(int B, int Tq, int Tk, int Hq, int Hk, int D, int uneven);
+size_t rs_attention_bwd_workspace_floats(int dtype, int B, int Tq, int Tk, int Hq, int Hk, int D, int uneven);
 int rs_attention_fwd(int dtype, const void* q, long long qb, long long qt, long long qh, const void* k, long long kb, long long kt,
                      long long kh, const void* v, long long vb, long long vt, long long vh, int B, int Tq, int Tk, int Hq, int Hk,
                      int D, const int* lengths, const int* query_lengths, int causal, const int* query_starts, int query_start,

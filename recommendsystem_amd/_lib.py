@@ -209,7 +209,7 @@ _PLAIN = {
     "rs_act_bwd_num_partials": (I, [L]),
     "rs_interact_partial_rows": (I, [I]),
     "rs_attention_fwd_workspace_floats": (SZ, [I, I, I, I, I, I, I]),
-    "rs_attention_bwd_workspace_floats": (SZ, [I, I, I, I, I, I, I]),
+    "rs_attention_bwd_workspace_floats": (SZ, [I, I, I, I, I, I, I, I]),
     "rs_layer_norm_partial_rows": (I, [I, I]),
     "rs_layer_norm_bwd_workspace_floats": (SZ, [I, I]),
     "rs_ffm_bwd_num_partials": (I, [I, I]),

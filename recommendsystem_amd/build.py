@@ -24,9 +24,9 @@ FLAGS = ["-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950", "-ffp-contract=o
          # no packed fp32 instructions: single fp32 operations everywhere (the host pass does not know the feature and
          # warns about it; the warning says nothing about the device code)
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-# Per-file additions.  interact.hip, attention.hip: MFMA results are consumed by vector instructions right away, so the products are
+# Per-file additions.  interact.hip, attention*.hip: MFMA results are consumed by vector instructions right away, so the products are
 # written to ordinary vector registers instead of accumulation registers that have to be copied out first.
-EXTRA_FLAGS = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for f in ("interact.hip", "attention.hip")}
+EXTRA_FLAGS = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for f in ("interact.hip", "attention.hip", "attention_small.hip")}
 
 
 def _newer(src: str, dst: str, deps) -> bool:

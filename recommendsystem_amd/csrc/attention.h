@@ -1,0 +1,95 @@
+// What the attention kernels share: their arguments, the mask, and how rows are read and written.
+#pragma once
+#include "lowp.h"
+
+struct AttnOperand {
+    const void* p;
+    long long b, t, h;      // strides in elements
+};
+
+struct AttnArgs {
+    AttnOperand q, k, v, o, go;                  // go: gradient of o
+    void *out, *dq, *dk, *dv;                // contiguous
+    float *lse, *delta;                      // [B, Hq, Tq]
+    const int *len, *qlen, *qstart;          // [B] or null
+    int B, Tq, Tk, Hk, G, D, causal, start;
+    float scale;
+    int tiles, splits;                       // row (key) tiles per (sample, key head); shares of the keys (rows)
+    int dealt;                               // order of the workgroups, see unit_of
+    // with splits > 1: forward [splits, B * Hk, Tq * G, D] and lse in base 2 [.., Tq * G], dk / dv [splits, 2, B, Tk, Hk, D]
+    float *part_o, *part_ml;
+    int vec;                                 // 16-byte loads from q, k, v, o, go
+    int out_vec;                             // four elements at once to the outputs
+};
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+typedef short rs_s16x4 __attribute__((ext_vector_type(4)));
+
+// E elements from column col of a row of D (zeros behind D, and everywhere when the row has no part).
+template <typename T, bool VEC> __device__ __forceinline__ typename RsVec<T>::V fetch(const T* row, int col, int D, bool live) {
+    typename RsVec<T>::V r;
+    constexpr int E = RsVec<T>::E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) r[e] = (T)0.f;
+    if (live && col < D) {
+        if constexpr (VEC) {
+            r = *(const typename RsVec<T>::V*)(row + col);
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (col + e < D) r[e] = row[col + e];
+        }
+    }
+    return r;
+}
+
+// A fragment that was loaded in front of a loop has arrived: without a use there, the wait for it would stand in the loop
+// and hold up the asynchronous loads, too.
+template <typename V> __device__ __forceinline__ void settle(V& v) {
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    union { V v; u32x4 u; } x;
+    x.v = v;
+    asm volatile("" : "+v"(x.u));
+    v = x.v;
+}
+// What a lane's row sees: keys below the result.
+__device__ __forceinline__ int row_limit(const AttnArgs& a, int b, int i) {
+    int lim = a.len ? min(max(a.len[b], 0), a.Tk) : a.Tk;
+    const int rows = a.qlen ? min(a.qlen[b], a.Tq) : a.Tq;
+    if (i >= rows) return 0;
+    if (a.causal) {
+        const long long last = (long long)i + (a.qstart ? a.qstart[b] : a.start) + 1;
+        lim = last < lim ? (last < 0 ? 0 : (int)last) : lim;
+    }
+    return lim;
+}
+
+template <typename T> __device__ __forceinline__ const T* row_ptr(const AttnOperand& x, int b, int t, int h) {
+    return (const T*)x.p + b * x.b + t * x.t + h * x.h;
+}
+
+// Four consecutive elements of an output row.
+template <typename T> __device__ __forceinline__ void store4(T* row, int d, int D, bool vec, const float* v) {
+    if (vec && d + 4 <= D) {
+        if constexpr (sizeof(T) == 4) {
+            *(rs_f32x4*)(row + d) = rs_f32x4{v[0], v[1], v[2], v[3]};
+        } else {
+            typedef T T4 __attribute__((ext_vector_type(4)));
+            *(T4*)(row + d) = T4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (d + e < D) row[d + e] = (T)v[e];
+    }
+}
+
+}  // namespace
+
+// Few keys (attention_small.hip): whether a call is for these kernels, and the two directions.
+bool rs_attention_small_ok(int dtype, int Tq, int Tk, int D);
+int rs_attention_small_fwd(int dtype, const AttnArgs& a, hipStream_t stream);
+int rs_attention_small_bwd(int dtype, const AttnArgs& a, hipStream_t stream);

@@ -25,36 +25,12 @@
 // Roundings: products of 16-bit operands are exact and summed in fp32; P and dS are rounded to the operands' type for
 // their second product (the matrix cores take equal types; the rounding is a half step per element and averages out over
 // the keys); all statistics, sums and outputs before their last rounding are fp32.
-#include "lowp.h"
+#include "attention.h"
 #include "../../include/rs_hip.h"
 
 #pragma clang fp contract(fast)
 
 namespace {
-
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-
-struct Operand {
-    const void* p;
-    long long b, t, h;      // strides in elements
-};
-
-struct AttnArgs {
-    Operand q, k, v, o, go;                  // go: gradient of o
-    void *out, *dq, *dk, *dv;                // contiguous
-    float *lse, *delta;                      // [B, Hq, Tq]
-    const int *len, *qlen, *qstart;          // [B] or null
-    int B, Tq, Tk, Hk, G, D, causal, start;
-    float scale;
-    int tiles, splits;                       // row (key) tiles per (sample, key head); shares of the keys (rows)
-    int dealt;                               // order of the workgroups, see unit_of
-    // with splits > 1: forward [splits, B * Hk, Tq * G, D] and lse in base 2 [.., Tq * G], dk / dv [splits, 2, B, Tk, Hk, D]
-    float *part_o, *part_ml;
-    int vec;                                 // 16-byte loads from q, k, v, o, go
-    int out_vec;                             // four elements at once to the outputs
-};
-
-typedef short rs_s16x4 __attribute__((ext_vector_type(4)));
 
 // Matrix tiles of one element type.  CK: elements of the contraction in one fragment pair; a fragment is 16 bytes a lane.
 template <typename T> struct Mma;
@@ -123,24 +99,6 @@ template <typename T, int DP> struct Tile {
     }
 };
 
-// E elements from column col of a row of D (zeros behind D, and everywhere when the row has no part).
-template <typename T, bool VEC> __device__ __forceinline__ typename Mma<T>::V fetch(const T* row, int col, int D, bool live) {
-    typename Mma<T>::V r;
-    constexpr int E = Mma<T>::E;
-#pragma unroll
-    for (int e = 0; e < E; ++e) r[e] = (T)0.f;
-    if (live && col < D) {
-        if constexpr (VEC) {
-            r = *(const typename Mma<T>::V*)(row + col);
-        } else {
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (col + e < D) r[e] = row[col + e];
-        }
-    }
-    return r;
-}
-
 // The way of consecutive tiles of R rows into LDS, NT lanes; rows from row_end on and columns from D on become zeros.
 // VEC: asynchronous 16-byte loads from memory to LDS through a buffer descriptor that ends with the last row, whose range
 // check supplies the zeros; no register holds the data, and the tile is there after the wait in feed_sync().
@@ -205,15 +163,6 @@ template <typename T, int DP, int R, int NT, bool VEC> struct Feed {
         }
     }
 };
-// A fragment that was loaded in front of a loop has arrived: without a use there, the wait for it would stand in the loop
-// and hold up the asynchronous loads, too.
-template <typename V> __device__ __forceinline__ void settle(V& v) {
-    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-    union { V v; u32x4 u; } x;
-    x.v = v;
-    asm volatile("" : "+v"(x.u));
-    v = x.v;
-}
 // This wave's loads have arrived and its reads are done, then everybody's.
 template <bool VEC> __device__ __forceinline__ void feed_sync() {
     if constexpr (VEC) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -258,38 +207,6 @@ inline long long order_units(AttnArgs& a) {      // the workgroups to launch for
     const long long pairs = (long long)a.B * a.Hk, per_pair = (long long)a.tiles * a.splits;
     a.dealt = pairs % 8 == 0 || pairs >= 64;
     return a.dealt ? (pairs + 7) / 8 * 8 * per_pair : (pairs * per_pair + 7) / 8 * 8;
-}
-
-// What a lane's row sees: keys below the result.
-__device__ __forceinline__ int row_limit(const AttnArgs& a, int b, int i) {
-    int lim = a.len ? min(max(a.len[b], 0), a.Tk) : a.Tk;
-    const int rows = a.qlen ? min(a.qlen[b], a.Tq) : a.Tq;
-    if (i >= rows) return 0;
-    if (a.causal) {
-        const long long last = (long long)i + (a.qstart ? a.qstart[b] : a.start) + 1;
-        lim = last < lim ? (last < 0 ? 0 : (int)last) : lim;
-    }
-    return lim;
-}
-
-template <typename T> __device__ __forceinline__ const T* row_ptr(const Operand& x, int b, int t, int h) {
-    return (const T*)x.p + b * x.b + t * x.t + h * x.h;
-}
-
-// Four consecutive elements of an output row.
-template <typename T> __device__ __forceinline__ void store4(T* row, int d, int D, bool vec, const float* v) {
-    if (vec && d + 4 <= D) {
-        if constexpr (sizeof(T) == 4) {
-            *(rs_f32x4*)(row + d) = rs_f32x4{v[0], v[1], v[2], v[3]};
-        } else {
-            typedef T T4 __attribute__((ext_vector_type(4)));
-            *(T4*)(row + d) = T4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (d + e < D) row[d + e] = (T)v[e];
-    }
 }
 
 template <typename T, int DP> constexpr int tile_rows() { return sizeof(T) == 4 && DP == 128 ? 32 : 64; }
@@ -871,11 +788,13 @@ bool shape_ok(const char* who, int dtype, int B, int Tq, int Tk, int Hq, int Hk,
     return true;
 }
 
-// 16-byte loads through a descriptor that ends with the last row: rows start at multiples of 16 bytes, do not overlap (T rows
-// of one sample; a single row has no stride), and a tile of them stays within 31 bits.
-bool operand_vec(const Operand& x, int dtype, int T, int D) {
+// An operand of T rows of D to a sample; the stride of a single row means nothing and becomes D.
+AttnOperand operand(const void* p, long long b, long long t, long long h, int T, int D) { return {p, b, T > 1 ? t : D, h}; }
+// 16-byte loads through a descriptor that ends with the last row: rows start at multiples of 16 bytes, do not overlap, and a
+// tile of them stays within 31 bits.
+bool operand_vec(const AttnOperand& x, int dtype, int D) {
     const int e = 16 / rs_elem_bytes(dtype);
-    return !x.p || (rs_aligned16(x.p) && x.b % e == 0 && x.h % e == 0 && (T <= 1 || (x.t % e == 0 && x.t >= D)) && x.t < (1 << 23));
+    return !x.p || (rs_aligned16(x.p) && x.b % e == 0 && x.h % e == 0 && x.t % e == 0 && x.t >= D && x.t < (1 << 23));
 }
 
 }  // namespace
@@ -884,6 +803,7 @@ extern "C" {
 
 size_t rs_attention_fwd_workspace_floats(int dtype, int B, int Tq, int Tk, int Hq, int Hk, int D) {
     if (B <= 0 || Tq <= 0 || Tk <= 0 || Hk < 1 || Hq < Hk || Hq % Hk || D < 1 || D > 128) return 0;
+    if (rs_attention_small_ok(dtype, Tq, Tk, D)) return 0;
     const int s = splits_for(dtype, B, Tq, Tk, Hk, Hq / Hk, D);
     return s == 1 ? 0 : (size_t)s * B * Tq * Hq * (D + 1);
 }
@@ -896,9 +816,9 @@ int rs_attention_fwd(int dtype, const void* q, long long qb, long long qt, long 
     if (B == 0 || Tq == 0) return RS_OK;
     RS_CHECK_ARG(q && o && (Tk == 0 || (k && v)), "rs_attention_fwd: null argument");
     AttnArgs a = {};
-    a.q = {q, qb, qt, qh};
-    a.k = {k, kb, kt, kh};
-    a.v = {v, vb, vt, vh};
+    a.q = operand(q, qb, qt, qh, Tq, D);
+    a.k = operand(k, kb, kt, kh, Tk, D);
+    a.v = operand(v, vb, vt, vh, Tk, D);
     a.out = o;
     a.lse = lse;
     a.len = lengths;
@@ -906,8 +826,9 @@ int rs_attention_fwd(int dtype, const void* q, long long qb, long long qt, long 
     a.qstart = query_starts;
     a.B = B, a.Tq = Tq, a.Tk = Tk, a.Hk = Hk, a.G = Hq / Hk, a.D = D, a.causal = causal != 0, a.start = query_start;
     a.scale = scale;
-    a.vec = D % (16 / rs_elem_bytes(dtype)) == 0 && operand_vec(a.q, dtype, Tq, D) && operand_vec(a.k, dtype, Tk, D) && operand_vec(a.v, dtype, Tk, D);
+    a.vec = D % (16 / rs_elem_bytes(dtype)) == 0 && operand_vec(a.q, dtype, D) && operand_vec(a.k, dtype, D) && operand_vec(a.v, dtype, D);
     a.out_vec = D % 4 == 0 && rs_aligned16(o);
+    if (rs_attention_small_ok(dtype, Tq, Tk, D)) return rs_attention_small_fwd(dtype, a, stream);
     const long long rows = (long long)Tq * a.G;
     const int nw = waves_for(rows);
     a.tiles = rs_cdiv(rows, nw * 32);
@@ -927,8 +848,9 @@ int rs_attention_fwd(int dtype, const void* q, long long qb, long long qt, long 
     return launch_fwd<_Float16>(a, nw, stream);
 }
 
-size_t rs_attention_bwd_workspace_floats(int B, int Tq, int Tk, int Hq, int Hk, int D, int uneven) {
+size_t rs_attention_bwd_workspace_floats(int dtype, int B, int Tq, int Tk, int Hq, int Hk, int D, int uneven) {
     if (B <= 0 || Tq <= 0 || Tk < 0 || Hk < 1 || Hq < Hk || Hq % Hk || D < 1 || D > 128) return 0;
+    if (rs_attention_small_ok(dtype, Tq, Tk, D)) return 0;
     const int s = Tk > 0 ? dkv_splits(B, Tq, Tk, Hk, Hq / Hk, uneven) : 1;
     // delta, up to a multiple of four floats, then the shares of dk and dv
     return ((size_t)B * Tq * Hq + 3) / 4 * 4 + (s > 1 ? (size_t)2 * s * B * Tk * Hk * D : 0);
@@ -944,18 +866,18 @@ int rs_attention_bwd(int dtype, const void* go, long long gb, long long gt, long
     if (B == 0 || (Tq == 0 && Tk == 0)) return RS_OK;
     RS_CHECK_ARG((Tq == 0 || (go && q && o && lse && dq)) && (Tk == 0 || (k && v && dk && dv)), "rs_attention_bwd: null argument");
     const int uneven = causal != 0 || lengths || query_lengths;
-    const size_t need = rs_attention_bwd_workspace_floats(B, Tq, Tk, Hq, Hk, D, uneven);
+    const size_t need = rs_attention_bwd_workspace_floats(dtype, B, Tq, Tk, Hq, Hk, D, uneven);
     if (need && (!workspace || workspace_floats < need)) {
         rs_set_error("rs_attention_bwd: workspace of %zu floats, %zu needed", workspace_floats, need);
         return RS_ERR_WORKSPACE;
     }
     RS_CHECK_ARG(rs_aligned16(workspace), "rs_attention_bwd: workspace must be aligned to 16 bytes");
     AttnArgs a = {};
-    a.q = {q, qb, qt, qh};
-    a.k = {k, kb, kt, kh};
-    a.v = {v, vb, vt, vh};
-    a.o = {o, ob, ot, oh};
-    a.go = {go, gb, gt, gh};
+    a.q = operand(q, qb, qt, qh, Tq, D);
+    a.k = operand(k, kb, kt, kh, Tk, D);
+    a.v = operand(v, vb, vt, vh, Tk, D);
+    a.o = operand(o, ob, ot, oh, Tq, D);
+    a.go = operand(go, gb, gt, gh, Tq, D);
     a.dq = dq, a.dk = dk, a.dv = dv;
     a.lse = (float*)lse;
     a.delta = workspace;
@@ -966,9 +888,10 @@ int rs_attention_bwd(int dtype, const void* go, long long gb, long long gt, long
     a.scale = scale;
     a.splits = Tq > 0 && Tk > 0 ? dkv_splits(B, Tq, Tk, Hk, a.G, uneven) : 1;
     a.part_o = workspace + ((size_t)B * Tq * Hq + 3) / 4 * 4;
-    a.vec = D % (16 / rs_elem_bytes(dtype)) == 0 && operand_vec(a.q, dtype, Tq, D) && operand_vec(a.k, dtype, Tk, D) && operand_vec(a.v, dtype, Tk, D) &&
-            operand_vec(a.o, dtype, Tq, D) && operand_vec(a.go, dtype, Tq, D);
+    a.vec = D % (16 / rs_elem_bytes(dtype)) == 0 && operand_vec(a.q, dtype, D) && operand_vec(a.k, dtype, D) && operand_vec(a.v, dtype, D) &&
+            operand_vec(a.o, dtype, D) && operand_vec(a.go, dtype, D);
     a.out_vec = D % 4 == 0 && rs_aligned16(dq) && rs_aligned16(dk) && rs_aligned16(dv);
+    if (rs_attention_small_ok(dtype, Tq, Tk, D)) return rs_attention_small_bwd(dtype, a, stream);
     if (dtype == RS_F32) return launch_bwd<float>(a, stream);
     if (dtype == RS_BF16) return launch_bwd<__bf16>(a, stream);
     return launch_bwd<_Float16>(a, stream);

@@ -2050,10 +2050,10 @@ def attention_bwd(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.T
     dk = torch.empty((B, Tk, Hk, D), dtype=q.dtype, device=dev)
     dv = torch.empty((B, Tk, Hk, D), dtype=q.dtype, device=dev)
     floats = _lib.lib().rs_attention_bwd_workspace_floats(
-        B, Tq, Tk, Hq, Hk, D, int(bool(causal) or lengths is not None or query_lengths is not None))
-    work = torch.empty(max(floats, 1), dtype=torch.float32, device=dev)
+        code, B, Tq, Tk, Hq, Hk, D, int(bool(causal) or lengths is not None or query_lengths is not None))
+    work = torch.empty(floats, dtype=torch.float32, device=dev) if floats else None
     gs, qs, ks, vs, os_ = do.stride(), q.stride(), k.stride(), v.stride(), o.stride()
     _call_on(dev, "rs_attention_bwd", code, do.data_ptr(), gs[0], gs[1], gs[2], q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0],
              ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2], o.data_ptr(), os_[0], os_[1], os_[2], lse.data_ptr(), B, Tq, Tk, Hq, Hk,
-             D, *how, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), work.data_ptr(), floats)
+             D, *how, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _addr(work), floats)
     return dq, dk, dv

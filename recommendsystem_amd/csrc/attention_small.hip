@@ -128,6 +128,18 @@ __device__ __forceinline__ int limit(const AttnArgs& a, const Part& p, int i) {
     return a.causal ? (int)min((long long)p.keys, p.start + i + 1) : p.keys;
 }
 
+// Workgroup -> (sample, head), sample >= B: none.  Workgroups go round the eight XCDs; the heads of a sample, whose rows
+// share cache lines (a head of 16 fp32 elements is half of one), go to one XCD where there are samples enough for all.
+struct Unit {
+    int b, h;
+};
+__device__ __forceinline__ Unit unit_of(const AttnArgs& a, int heads) {
+    const unsigned id = (unsigned)rs_block_id(), n = heads;
+    if (!a.dealt) return {(int)(id / n), (int)(id % n)};
+    const unsigned j = id >> 3, k = j / n;
+    return {(int)(k * 8 + (id & 7)), (int)(j - k * n)};
+}
+
 // ---- forward -----------------------------------------------------------------------------------------------------
 // NT: tiles of 16 keys.  A workgroup is one wave with one head of one sample.
 template <typename T, int DP, int NT, bool VEC>
@@ -137,10 +149,10 @@ __global__ __launch_bounds__(64) void attention_small_fwd_kernel(const AttnArgs 
     typedef Rows<T, DP> L;
     __shared__ __align__(16) T s_k[NT * 16 * L::RS];
     __shared__ __align__(16) T s_v[NT * 16 * L::RS];
-    const long long unit = rs_block_id();
     const int Hq = a.Hk * a.G;
-    if (unit >= (long long)a.B * Hq) return;
-    const int b = (unsigned)unit / (unsigned)Hq, h = (unsigned)unit % (unsigned)Hq, hk = (unsigned)h / (unsigned)a.G;
+    const Unit unit = unit_of(a, Hq);
+    if (unit.b >= a.B) return;
+    const int b = unit.b, h = unit.h, hk = (unsigned)h / (unsigned)a.G;
     const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
     const Part part = part_of(a, b);
     const float scale2 = a.scale * LOG2E;
@@ -220,9 +232,9 @@ __global__ __launch_bounds__(64) void attention_small_bwd_kernel(const AttnArgs 
     __shared__ __align__(16) T s_g[R * L::RS];
     __shared__ __align__(16) T s_p[R * LP::RS];
     __shared__ __align__(16) T s_d[R * LP::RS];
-    const long long unit = rs_block_id();
-    if (unit >= (long long)a.B * a.Hk) return;
-    const int b = (unsigned)unit / (unsigned)a.Hk, hk = (unsigned)unit % (unsigned)a.Hk, Hq = a.Hk * a.G;
+    const Unit unit = unit_of(a, a.Hk);
+    if (unit.b >= a.B) return;
+    const int b = unit.b, hk = unit.h, Hq = a.Hk * a.G;
     const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
     const Part part = part_of(a, b);
     const float scale2 = a.scale * LOG2E;
@@ -339,8 +351,9 @@ __global__ __launch_bounds__(64) void attention_small_bwd_kernel(const AttnArgs 
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------
-template <typename T, int DP, int NT> int launch(const AttnArgs& a, bool back, hipStream_t stream) {
-    const dim3 grid = rs_grid((long long)a.B * a.Hk * (back ? 1 : a.G));
+template <typename T, int DP, int NT> int launch(AttnArgs a, bool back, hipStream_t stream) {
+    a.dealt = a.B >= 64;
+    const dim3 grid = rs_grid((a.dealt ? (a.B + 7LL) / 8 * 8 : a.B) * a.Hk * (back ? 1 : a.G));
     if (back && a.vec) hipLaunchKernelGGL((attention_small_bwd_kernel<T, DP, NT, true>), grid, dim3(64), 0, stream, a);
     else if (back) hipLaunchKernelGGL((attention_small_bwd_kernel<T, DP, NT, false>), grid, dim3(64), 0, stream, a);
     else if (a.vec) hipLaunchKernelGGL((attention_small_fwd_kernel<T, DP, NT, true>), grid, dim3(64), 0, stream, a);

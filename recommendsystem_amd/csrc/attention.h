@@ -37,6 +37,8 @@ template <typename T, bool VEC> __device__ __forceinline__ typename RsVec<T>::V 
     if (live && col < D) {
         if constexpr (VEC) {
             r = *(const typename RsVec<T>::V*)(row + col);
+        } else if (col + E <= D) {
+            r = *(const typename RsVec<T>::U*)(row + col);
         } else {
 #pragma unroll
             for (int e = 0; e < E; ++e)

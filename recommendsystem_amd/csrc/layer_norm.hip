@@ -4,9 +4,9 @@
 //   dw = sum_rows dy xhat,  db = sum_rows dy
 // All statistics and sums are fp32; the variance is that of the centred values (no E[x^2] - mean^2 cancellation).
 //
-// Both directions are bound by memory: a row is read once into registers by LPR lanes that own 16 elements each (as
-// 16-byte vectors where N, the strides and the addresses allow, else single elements), reduced across those lanes and
-// written once.  LPR is the smallest of 8, 32, 64, 256 and 1024 that covers the row: rows of up to 1024 elements need no
+// Both directions are bound by memory: a row is read once into registers by LPR lanes that own 16 elements each, as 16-byte
+// vectors (WHOLE: aligned ones, where N, the strides and the addresses allow; else at any address, the row's last vector
+// element by element), reduced across those lanes and written once.  LPR is the smallest of 8, 32, 64, 256 and 1024 that covers the row: rows of up to 1024 elements need no
 // workgroup barrier, and a workgroup holds 256 / LPR rows at a time.  Rows beyond 16384 elements go through a
 // workgroup of 1024 that reads them again from the caches for each pass.
 //
@@ -51,34 +51,29 @@ template <int LPR> __device__ __forceinline__ float2 row_sum2(float a, float b, 
     return make_float2(a, b);
 }
 
-// VE weights (or biases) at column n: their type is T or fp32; absent ones are `other`.
-template <typename T, int VE> __device__ __forceinline__ void load_param(const void* p, int is_f32, int n, float other, float* v) {
+// E weights (or biases) from column n on: their type is T or fp32; absent ones are `other`.
+template <typename T, bool WHOLE> __device__ __forceinline__ void load_param(const void* p, int is_f32, int n, int left, float other, float* v) {
+    constexpr int E = RsVec<T>::E;
     if (!p) {
 #pragma unroll
-        for (int e = 0; e < VE; ++e) v[e] = other;
+        for (int e = 0; e < E; ++e) v[e] = other;
     } else if (is_f32) {
-        const float* f = (const float*)p + n;
-        if constexpr (VE == 1) {
-            v[0] = f[0];
-        } else {
 #pragma unroll
-            for (int q = 0; q < VE / 4; ++q) {
-                const rs_f32x4 x = *(const rs_f32x4*)(f + 4 * q);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[4 * q + e] = x[e];
-            }
-        }
+        for (int q = 0; q < E; q += 4) rs_load<float, WHOLE>((const float*)p + n + q, left - q, v + q);
     } else {
-        rs_load<T, VE>((const T*)p + n, v);
+        rs_load<T, WHOLE>((const T*)p + n, left, v);
     }
 }
+template <typename T> __device__ __forceinline__ float one_param(const void* p, int is_f32, int n, float other) {
+    return !p ? other : is_f32 ? ((const float*)p)[n] : (float)((const T*)p)[n];
+}
 
-template <typename T, int VE, int LPR>
+template <typename T, bool WHOLE, int LPR>
 __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void layer_norm_fwd_kernel(
     const T* __restrict__ x, long long ldx, const T* __restrict__ r, long long ldr, int M, int N, const void* __restrict__ w,
     const void* __restrict__ b, int param_f32, float eps, T* __restrict__ y, T* __restrict__ s_out,
     float* __restrict__ mean_out, float* __restrict__ rstd_out) {
-    constexpr int NT = LPR > 256 ? LPR : 256, CH = EPT / VE;
+    constexpr int NT = LPR > 256 ? LPR : 256, VE = RsVec<T>::E, CH = EPT / VE;
     __shared__ float red[2][NT / 64];
     const int t = threadIdx.x % LPR;
     const long long m = rs_block_id() * (NT / LPR) + threadIdx.x / LPR;
@@ -90,13 +85,13 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void layer_norm_fwd_kernel(
         const int n = (c * LPR + t) * VE;
         float* vc = v + c * VE;
         if (live && n < N) {
-            rs_load<T, VE>(x + m * ldx + n, vc);
+            rs_load<T, WHOLE>(x + m * ldx + n, N - n, vc);
             if (r) {
                 float q[VE];
-                rs_load<T, VE>(r + m * ldr + n, q);
+                rs_load<T, WHOLE>(r + m * ldr + n, N - n, q);
 #pragma unroll
                 for (int e = 0; e < VE; ++e) vc[e] = (float)(T)(vc[e] + q[e]);      // s is what its type holds
-                rs_store<T, VE>(s_out + m * N + n, vc);
+                rs_store<T, WHOLE>(s_out + m * N + n, N - n, vc);
             }
 #pragma unroll
             for (int e = 0; e < VE; ++e) sum += vc[e];
@@ -110,7 +105,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void layer_norm_fwd_kernel(
 #pragma unroll
             for (int e = 0; e < VE; ++e) {
                 const float d = v[c * VE + e] - mu;
-                sq += d * d;
+                if (WHOLE || (c * LPR + t) * VE + e < N) sq += d * d;
             }
     const float rstd = 1.f / sqrtf(row_sum<LPR>(sq, red[1]) / (float)N + eps);
     if (!live) return;
@@ -123,11 +118,11 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void layer_norm_fwd_kernel(
         const int n = (c * LPR + t) * VE;
         if (n < N) {
             float wv[VE], bv[VE], o[VE];
-            load_param<T, VE>(w, param_f32, n, 1.f, wv);
-            load_param<T, VE>(b, param_f32, n, 0.f, bv);
+            load_param<T, WHOLE>(w, param_f32, n, N - n, 1.f, wv);
+            load_param<T, WHOLE>(b, param_f32, n, N - n, 0.f, bv);
 #pragma unroll
             for (int e = 0; e < VE; ++e) o[e] = (v[c * VE + e] - mu) * rstd * wv[e] + bv[e];
-            rs_store<T, VE>(y + m * N + n, o);
+            rs_store<T, WHOLE>(y + m * N + n, N - n, o);
         }
     }
 }
@@ -164,20 +159,17 @@ __global__ __launch_bounds__(1024) void layer_norm_fwd_long_kernel(
         if (rstd_out) rstd_out[m] = rstd;
     }
     for (int n = threadIdx.x; n < N; n += 1024) {
-        float wv, bv;
-        load_param<T, 1>(w, param_f32, n, 1.f, &wv);
-        load_param<T, 1>(b, param_f32, n, 0.f, &bv);
-        y[m * N + n] = (T)(((float)row[n] - mu) * rstd * wv + bv);
+        y[m * N + n] = (T)(((float)row[n] - mu) * rstd * one_param<T>(w, param_f32, n, 1.f) + one_param<T>(b, param_f32, n, 0.f));
     }
 }
 
 // part: [gridDim.x, 2, N], dw sums in front of db sums.
-template <typename T, int VE, int LPR>
+template <typename T, bool WHOLE, int LPR>
 __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void layer_norm_bwd_kernel(
     const T* __restrict__ dy, long long lddy, const T* __restrict__ s, long long lds, const float* __restrict__ mean,
     const float* __restrict__ rstd, const void* __restrict__ w, int param_f32, const T* __restrict__ ds, long long ldds, int M,
     int N, T* __restrict__ dx, float* __restrict__ part) {
-    constexpr int NT = LPR > 256 ? LPR : 256, CH = EPT / VE, R = NT / LPR;
+    constexpr int NT = LPR > 256 ? LPR : 256, VE = RsVec<T>::E, CH = EPT / VE, R = NT / LPR;
     __shared__ float red[2][2 * (NT / 64)];
     __shared__ float fold[R > 1 ? R * LPR : 1];
     const int t = threadIdx.x % LPR, g = threadIdx.x / LPR;
@@ -187,7 +179,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void layer_norm_bwd_kernel(
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int n = (c * LPR + t) * VE;
-        if (n < N) load_param<T, VE>(w, param_f32, n, 1.f, wv + c * VE);
+        if (n < N) load_param<T, WHOLE>(w, param_f32, n, N - n, 1.f, wv + c * VE);
     }
     const float inv = 1.f / (float)N;
     int turn = 0;
@@ -204,8 +196,8 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void layer_norm_bwd_kernel(
             float* xc = xh + c * VE;
             float* gc = gy + c * VE;
             if (live && n < N) {
-                rs_load<T, VE>(s + m * lds + n, xc);
-                rs_load<T, VE>(dy + m * lddy + n, gc);
+                rs_load<T, WHOLE>(s + m * lds + n, N - n, xc);
+                rs_load<T, WHOLE>(dy + m * lddy + n, N - n, gc);
 #pragma unroll
                 for (int e = 0; e < VE; ++e) {
                     xc[e] = (xc[e] - mu) * rs;
@@ -228,11 +220,11 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void layer_norm_bwd_kernel(
                 for (int e = 0; e < VE; ++e) o[e] = rs * (gy[c * VE + e] - c1 - xh[c * VE + e] * c2);
                 if (ds) {
                     float q[VE];
-                    rs_load<T, VE>(ds + m * ldds + n, q);
+                    rs_load<T, WHOLE>(ds + m * ldds + n, N - n, q);
 #pragma unroll
                     for (int e = 0; e < VE; ++e) o[e] += q[e];
                 }
-                rs_store<T, VE>(dx + m * N + n, o);
+                rs_store<T, WHOLE>(dx + m * N + n, N - n, o);
             }
         }
     }
@@ -281,8 +273,7 @@ __global__ __launch_bounds__(1024) void layer_norm_bwd_long_kernel(
         float s1 = 0.f, s2 = 0.f;
         for (int n = threadIdx.x; n < N; n += 1024) {
             const float xh = ((float)s[m * lds + n] - mu) * rs, d = (float)dy[m * lddy + n];
-            float wv;
-            load_param<T, 1>(w, param_f32, n, 1.f, &wv);
+            const float wv = one_param<T>(w, param_f32, n, 1.f);
             s1 += d * wv;
             s2 += d * wv * xh;
             if (pw) {                        // a column belongs to one lane: no other touches its sums
@@ -294,9 +285,7 @@ __global__ __launch_bounds__(1024) void layer_norm_bwd_long_kernel(
         const float c1 = sums.x * inv, c2 = sums.y * inv;
         for (int n = threadIdx.x; n < N; n += 1024) {
             const float xh = ((float)s[m * lds + n] - mu) * rs;
-            float wv;
-            load_param<T, 1>(w, param_f32, n, 1.f, &wv);
-            float o = rs * ((float)dy[m * lddy + n] * wv - c1 - xh * c2);
+            float o = rs * ((float)dy[m * lddy + n] * one_param<T>(w, param_f32, n, 1.f) - c1 - xh * c2);
             if (ds) o += (float)ds[m * ldds + n];
             dx[m * N + n] = (T)o;
         }
@@ -346,18 +335,18 @@ struct NormArgs {
     float *mean, *rstd;
 };
 
-// 16-byte accesses need every row of every operand to start at a multiple of 16 bytes.
+// Aligned 16-byte accesses need every row of every operand to start at a multiple of 16 bytes.
 inline bool vec_ok(int dtype, int N, long long ld, const void* p) {
     const int e = 16 / rs_elem_bytes(dtype);
     return !p || (rs_aligned16(p) && ld % e == 0 && N % e == 0);
 }
 
-template <typename T, int VE> int launch_fwd(const NormArgs& a, hipStream_t stream) {
+template <typename T, bool WHOLE> int launch_fwd(const NormArgs& a, hipStream_t stream) {
     const int l = lanes_for(a.N);
     const T *x = (const T*)a.x, *r = (const T*)a.r;
 #define RS_LN_FWD(L)                                                                                                          \
     case L:                                                                                                                   \
-        hipLaunchKernelGGL((layer_norm_fwd_kernel<T, VE, L>), rs_grid(rs_cdiv(a.M, (L > 256 ? L : 256) / L)),                 \
+        hipLaunchKernelGGL((layer_norm_fwd_kernel<T, WHOLE, L>), rs_grid(rs_cdiv(a.M, (L > 256 ? L : 256) / L)),                 \
                            dim3(L > 256 ? L : 256), 0, stream, x, a.ldx, r, a.ldr, a.M, a.N, a.w, a.b, a.param_f32, a.eps,    \
                            (T*)a.y, (T*)a.s, a.mean, a.rstd);                                                                 \
         break;
@@ -377,13 +366,13 @@ template <typename T, int VE> int launch_fwd(const NormArgs& a, hipStream_t stre
 }
 
 // y = dy, s, ds as inputs; b unused
-template <typename T, int VE> int launch_bwd(const NormArgs& a, const void* dy, long long lddy, void* dx, float* part, int rows,
+template <typename T, bool WHOLE> int launch_bwd(const NormArgs& a, const void* dy, long long lddy, void* dx, float* part, int rows,
                                              hipStream_t stream) {
     const int l = lanes_for(a.N);
     const T *s = (const T*)a.x, *d = (const T*)dy, *ds = (const T*)a.ds;
 #define RS_LN_BWD(L)                                                                                                          \
     case L:                                                                                                                   \
-        hipLaunchKernelGGL((layer_norm_bwd_kernel<T, VE, L>), dim3(rows), dim3(L > 256 ? L : 256), 0, stream, d, lddy, s,      \
+        hipLaunchKernelGGL((layer_norm_bwd_kernel<T, WHOLE, L>), dim3(rows), dim3(L > 256 ? L : 256), 0, stream, d, lddy, s,      \
                            a.ldx, a.mean, a.rstd, a.w, a.param_f32, ds, a.ldds, a.M, a.N, (T*)dx, part);                      \
         break;
     switch (l) {
@@ -430,9 +419,9 @@ int rs_layer_norm_fwd(int dtype, int param_dtype, const void* x, long long ldx, 
     const NormArgs a = {x, r, w, b, nullptr, ldx, ldr, 0, M, N, param_dtype == RS_F32, eps, y, s, mean, rstd};
     const bool vec = vec_ok(dtype, N, M > 1 ? ldx : 0, x) && vec_ok(dtype, N, M > 1 ? ldr : 0, r) && rs_aligned16(y) &&
                      (!r || rs_aligned16(s)) && rs_aligned16(w) && rs_aligned16(b);
-    if (dtype == RS_F32) return vec ? launch_fwd<float, 4>(a, stream) : launch_fwd<float, 1>(a, stream);
-    if (dtype == RS_BF16) return vec ? launch_fwd<__bf16, 8>(a, stream) : launch_fwd<__bf16, 1>(a, stream);
-    return vec ? launch_fwd<_Float16, 8>(a, stream) : launch_fwd<_Float16, 1>(a, stream);
+    if (dtype == RS_F32) return vec ? launch_fwd<float, true>(a, stream) : launch_fwd<float, false>(a, stream);
+    if (dtype == RS_BF16) return vec ? launch_fwd<__bf16, true>(a, stream) : launch_fwd<__bf16, false>(a, stream);
+    return vec ? launch_fwd<_Float16, true>(a, stream) : launch_fwd<_Float16, false>(a, stream);
 }
 
 int rs_layer_norm_bwd(int dtype, int param_dtype, const void* dy, long long lddy, const void* s, long long lds,
@@ -458,14 +447,14 @@ int rs_layer_norm_bwd(int dtype, int param_dtype, const void* dy, long long lddy
                          vec_ok(dtype, N, M > 1 ? ldds : 0, ds) && rs_aligned16(dx) && rs_aligned16(w);
         int rc;
         if (dtype == RS_F32)
-            rc = vec ? launch_bwd<float, 4>(a, dy, lddy, dx, part, rows, stream)
-                     : launch_bwd<float, 1>(a, dy, lddy, dx, part, rows, stream);
+            rc = vec ? launch_bwd<float, true>(a, dy, lddy, dx, part, rows, stream)
+                     : launch_bwd<float, false>(a, dy, lddy, dx, part, rows, stream);
         else if (dtype == RS_BF16)
-            rc = vec ? launch_bwd<__bf16, 8>(a, dy, lddy, dx, part, rows, stream)
-                     : launch_bwd<__bf16, 1>(a, dy, lddy, dx, part, rows, stream);
+            rc = vec ? launch_bwd<__bf16, true>(a, dy, lddy, dx, part, rows, stream)
+                     : launch_bwd<__bf16, false>(a, dy, lddy, dx, part, rows, stream);
         else
-            rc = vec ? launch_bwd<_Float16, 8>(a, dy, lddy, dx, part, rows, stream)
-                     : launch_bwd<_Float16, 1>(a, dy, lddy, dx, part, rows, stream);
+            rc = vec ? launch_bwd<_Float16, true>(a, dy, lddy, dx, part, rows, stream)
+                     : launch_bwd<_Float16, false>(a, dy, lddy, dx, part, rows, stream);
         if (rc != RS_OK) return rc;
     }
     if (params) {                            // no rows: the sums are zero

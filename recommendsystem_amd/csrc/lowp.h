@@ -9,31 +9,51 @@ typedef float rs_f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 rs_bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 rs_f16x8 __attribute__((ext_vector_type(8)));
 
-// V = the 16-byte vector of T, E = its elements.
+// V = the 16-byte vector of T, U = the same at any address, E = its elements.
 template <typename T> struct RsVec;
-template <> struct RsVec<float> { typedef rs_f32x4 V; static constexpr int E = 4; };
-template <> struct RsVec<__bf16> { typedef rs_bf16x8 V; static constexpr int E = 8; };
-template <> struct RsVec<_Float16> { typedef rs_f16x8 V; static constexpr int E = 8; };
+template <> struct RsVec<float> {
+    typedef rs_f32x4 V;
+    typedef rs_f32x4 U __attribute__((aligned(4)));
+    static constexpr int E = 4;
+};
+template <> struct RsVec<__bf16> {
+    typedef rs_bf16x8 V;
+    typedef rs_bf16x8 U __attribute__((aligned(2)));
+    static constexpr int E = 8;
+};
+template <> struct RsVec<_Float16> {
+    typedef rs_f16x8 V;
+    typedef rs_f16x8 U __attribute__((aligned(2)));
+    static constexpr int E = 8;
+};
 
-// VE consecutive elements as fp32: one 16-byte access (VE = RsVec<T>::E, p aligned to 16 bytes) or a single one.
-// Stores round to nearest even once.
-template <typename T, int VE> __device__ __forceinline__ void rs_load(const T* p, float* v) {
-    if constexpr (VE == 1) {
-        v[0] = (float)*p;
-    } else {
-        const typename RsVec<T>::V x = *(const typename RsVec<T>::V*)p;
+// E consecutive elements as fp32, in one 16-byte access.  WHOLE: p is aligned to 16 bytes and all E elements are there; else
+// p is any element and the first `left` of E belong to the row (zeros for the others).  Stores round to nearest even once.
+template <typename T, bool WHOLE> __device__ __forceinline__ void rs_load(const T* p, int left, float* v) {
+    constexpr int E = RsVec<T>::E;
+    if (WHOLE || left >= E) {
+        typename RsVec<T>::V x;
+        if constexpr (WHOLE) x = *(const typename RsVec<T>::V*)p;
+        else x = *(const typename RsVec<T>::U*)p;
 #pragma unroll
-        for (int e = 0; e < VE; ++e) v[e] = (float)x[e];
+        for (int e = 0; e < E; ++e) v[e] = (float)x[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = e < left ? (float)p[e] : 0.f;
     }
 }
-template <typename T, int VE> __device__ __forceinline__ void rs_store(T* p, const float* v) {
-    if constexpr (VE == 1) {
-        *p = (T)v[0];
-    } else {
+template <typename T, bool WHOLE> __device__ __forceinline__ void rs_store(T* p, int left, const float* v) {
+    constexpr int E = RsVec<T>::E;
+    if (WHOLE || left >= E) {
         typename RsVec<T>::V x;
 #pragma unroll
-        for (int e = 0; e < VE; ++e) x[e] = (T)v[e];
-        *(typename RsVec<T>::V*)p = x;
+        for (int e = 0; e < E; ++e) x[e] = (T)v[e];
+        if constexpr (WHOLE) *(typename RsVec<T>::V*)p = x;
+        else *(typename RsVec<T>::U*)p = x;
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (e < left) p[e] = (T)v[e];
     }
 }
 

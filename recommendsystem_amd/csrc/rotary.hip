@@ -31,6 +31,16 @@ struct RotaryArgs {
     int per_block;                         // tokens of a workgroup
 };
 
+// VE elements: an aligned 16-byte vector or one element.
+template <typename T, int VE> __device__ __forceinline__ void load(const T* p, float* v) {
+    if constexpr (VE == 1) v[0] = (float)*p;
+    else rs_load<T, true>(p, VE, v);
+}
+template <typename T, int VE> __device__ __forceinline__ void store(T* p, const float* v) {
+    if constexpr (VE == 1) *p = (T)v[0];
+    else rs_store<T, true>(p, VE, v);
+}
+
 template <typename T, int VE, bool PAIRED>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
     __shared__ int s_pos[TOKENS_MAX];
@@ -70,16 +80,16 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
         if constexpr (!PAIRED) {
             const unsigned n = u * VE;
             float x[VE], y[VE], p[VE], q[VE];
-            rs_load<T, VE>(in + n, x);
-            rs_load<T, VE>(in + half + n, y);
+            load<T, VE>(in + n, x);
+            load<T, VE>(in + half + n, y);
 #pragma unroll
             for (int e = 0; e < VE; ++e) {
                 const float c = cs[n + e], s = sn[n + e] * a.sign;
                 p[e] = x[e] * c - y[e] * s;
                 q[e] = y[e] * c + x[e] * s;
             }
-            rs_store<T, VE>(out + n, p);
-            rs_store<T, VE>(out + half + n, q);
+            store<T, VE>(out + n, p);
+            store<T, VE>(out + half + n, q);
         } else if constexpr (VE == 1) {
             const float x = (float)in[2 * u], y = (float)in[2 * u + 1], c = cs[u], s = sn[u] * a.sign;
             out[2 * u] = (T)(x * c - y * s);
@@ -87,14 +97,14 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
         } else {
             const unsigned n = u * VE;
             float x[VE];
-            rs_load<T, VE>(in + n, x);
+            load<T, VE>(in + n, x);
 #pragma unroll
             for (int e = 0; e < VE; e += 2) {
                 const float c = cs[(n + e) / 2], s = sn[(n + e) / 2] * a.sign, v = x[e];
                 x[e] = v * c - x[e + 1] * s;
                 x[e + 1] = x[e + 1] * c + v * s;
             }
-            rs_store<T, VE>(out + n, x);
+            store<T, VE>(out + n, x);
         }
     }
 }

@@ -89,6 +89,39 @@ template <typename T> __device__ __forceinline__ void store4(T* row, int d, int 
     }
 }
 
+// 16x16 tiles: CK elements of the contraction in a fragment pair, 16 bytes a lane; lane l holds row (column) l % 16 and
+// elements E (l / 16) .. of the CK.  A result holds column l % 16 and rows 4 (l / 16) + 0..3.
+template <typename T> struct Mma16;
+template <> struct Mma16<float> {
+    static constexpr int CK = 16, E = 4, TILES = 1;          // TILES: row tiles that one contraction step over rows covers
+    typedef rs_f32x4 V;
+    static __device__ __forceinline__ rs_f32x4 mul(V a, V b, rs_f32x4 c) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+        return c;
+    }
+};
+template <> struct Mma16<__bf16> {
+    static constexpr int CK = 32, E = 8, TILES = 2;
+    typedef rs_bf16x8 V;
+    static __device__ __forceinline__ rs_f32x4 mul(V a, V b, rs_f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mma16<_Float16> {
+    static constexpr int CK = 32, E = 8, TILES = 2;
+    typedef rs_f16x8 V;
+    static __device__ __forceinline__ rs_f32x4 mul(V a, V b, rs_f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+
+// Over the four lanes that hold a column.
+__device__ __forceinline__ float col_max(float x) {
+    x = fmaxf(x, __shfl_xor(x, 16, 64));
+    return fmaxf(x, __shfl_xor(x, 32, 64));
+}
+__device__ __forceinline__ float col_sum(float x) {
+    x += __shfl_xor(x, 16, 64);
+    return x + __shfl_xor(x, 32, 64);
+}
+
 }  // namespace
 
 // Few keys (attention_small.hip): whether a call is for these kernels, and the two directions.

@@ -357,6 +357,125 @@ __global__ __launch_bounds__(NW * 64) void attention_fwd_kernel(const AttnArgs a
         }
 }
 
+// At most 16 rows (single tokens, short chunks) in fp32, whose matrix instructions are slow enough to matter here: 16x16 tiles
+// do half the work of 32x32 ones padded from 16 columns (531 samples x 4 rows x 2 heads of 96 over caches of up to 7632:
+// 1155 -> 509 us, 3.0 TB/s; 64 tokens x 8 heads of 128 over 4096 keys each 390 us, 5.5 TB/s).  One wave, 16 or 32 keys at
+// a time; as above otherwise.
+template <int DP, int KT, bool VEC>
+__global__ __launch_bounds__(64) void attention_few_fwd_kernel(const AttnArgs a) {
+    typedef float T;
+    constexpr int CK = Mma16<T>::CK, E = Mma16<T>::E, NC = DP / CK, ND = DP / 16, NK = KT / 16;
+    typedef typename Mma16<T>::V V;
+    typedef Tile<T, DP> L;
+    __shared__ __align__(1024) T s_k[2][KT * DP];
+    __shared__ __align__(1024) T s_v[2][KT * DP];
+    const Unit unit = unit_of(a);
+    if (unit.pair < 0) return;
+    const int split = unit.split, pair = unit.pair, b = pair / a.Hk, hk = pair % a.Hk;
+    const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+    const int rows = a.Tq * a.G, i = (unsigned)col / (unsigned)a.G, h = hk * a.G + (unsigned)col % (unsigned)a.G;
+    const bool live = col < rows;
+    const int lim = live ? row_limit(a, b, i) : 0;
+    int end = lim, low = lim;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+        end = max(end, __shfl_xor(end, o, 64));
+        low = min(low, __shfl_xor(low, o, 64));
+    }
+    end = __builtin_amdgcn_readfirstlane(end);
+    low = __builtin_amdgcn_readfirstlane(low);
+    int k0 = 0;
+    if (a.splits > 1) {
+        const int per = ((end + KT - 1) / KT + a.splits - 1) / a.splits * KT;
+        k0 = min(split * per, end);
+        end = min(k0 + per, end);
+    }
+    V qf[NC];
+    const T* qr = row_ptr<T>(a.q, b, live ? i : 0, live ? h : 0);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) qf[c] = fetch<T, VEC>(qr, c * CK + g * E, a.D, lim > 0);
+    rs_f32x4 acc[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) acc[d] = rs_f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+    const float scale2 = a.scale * LOG2E;
+    Feed<T, DP, KT, 64, VEC> fk(a.k.t, a.D), fv(a.v.t, a.D);
+    fk.seek(row_ptr<T>(a.k, b, 0, hk), k0, end);
+    fv.seek(row_ptr<T>(a.v, b, 0, hk), k0, end);
+    if (k0 < end) {
+        fk.next(s_k[0]);
+        fv.next(s_v[0]);
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) settle(qf[c]);
+    for (int buf = 0; k0 < end; k0 += KT, buf ^= 1) {
+        fk.land(s_k[buf]);
+        fv.land(s_v[buf]);
+        feed_sync<VEC>();
+        if (k0 + KT < end) {
+            fk.next(s_k[buf ^ 1]);
+            fv.next(s_v[buf ^ 1]);
+        }
+        rs_f32x4 s[NK];
+        float top = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < NK; ++n) {
+            s[n] = rs_f32x4{0.f, 0.f, 0.f, 0.f};
+            const int r = n * 16 + col;
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+                s[n] = Mma16<T>::mul(*(const V*)(s_k[buf] + r * DP + ((c * 4 + g) ^ L::swz(r)) * E), qf[c], s[n]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (k0 + KT > low && k0 + n * 16 + 4 * g + e >= lim) s[n][e] = -INFINITY;
+                top = fmaxf(top, s[n][e]);
+            }
+        }
+        const float m_new = fmaxf(m, col_max(top) * scale2), base = m_new == -INFINITY ? 0.f : m_new;
+        const float alpha = __builtin_amdgcn_exp2f(m - base);
+        m = m_new;
+        l *= alpha;                                               // this lane's keys only
+#pragma unroll
+        for (int n = 0; n < NK; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                s[n][e] = __builtin_amdgcn_exp2f(s[n][e] * scale2 - base);
+                l += s[n][e];
+            }
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[d][e] *= alpha;
+#pragma unroll
+            for (int n = 0; n < NK; ++n) {
+                V v;
+                const int at = d * 16 + col;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const int r = n * 16 + 4 * g + x;
+                    v[x] = s_v[buf][r * DP + ((at / E) ^ L::swz(r)) * E + at % E];
+                }
+                acc[d] = Mma16<T>::mul(v, s[n], acc[d]);
+            }
+        }
+    }
+    l = col_sum(l);
+    if (!live) return;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const bool shared_out = a.splits > 1;
+    const long long at = ((long long)split * a.B * a.Hk + pair) * rows + col;
+    T* out = shared_out ? a.part_o + at * a.D : (T*)a.out + (((long long)b * a.Tq + i) * a.Hk * a.G + h) * a.D;
+    if (g == 0) {
+        if (shared_out) a.part_ml[at] = l == 0.f ? -INFINITY : m + log2f(l);
+        else if (a.lse) a.lse[((long long)b * a.Hk * a.G + h) * a.Tq + i] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+    }
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+        const float x[4] = {acc[d][0] * inv, acc[d][1] * inv, acc[d][2] * inv, acc[d][3] * inv};
+        store4<T>(out, d * 16 + 4 * g, a.D, shared_out ? a.D % 4 == 0 : a.out_vec, x);
+    }
+}
+
 // Joins the shares of a row: weights exp2(lse_s - max) over their sum.  A wave to a row.
 template <typename T> __global__ __launch_bounds__(256) void attention_join_kernel(const AttnArgs a) {
     const long long rows = (long long)a.Tq * a.G, all = rows * a.B * a.Hk;
@@ -717,8 +836,14 @@ int dkv_splits(int B, int Tq, int Tk, int Hk, int G, int uneven) {
 template <typename T, int DP, int NW> int launch_fwd(AttnArgs a, hipStream_t stream) {
     constexpr int KT = NW == 1 ? 32 : tile_rows<T, DP>();
     const dim3 grid = rs_grid(order_units(a));
-    if (a.vec) hipLaunchKernelGGL((attention_fwd_kernel<T, DP, NW, KT, true>), grid, dim3(NW * 64), 0, stream, a);
-    else hipLaunchKernelGGL((attention_fwd_kernel<T, DP, NW, KT, false>), grid, dim3(NW * 64), 0, stream, a);
+    const bool few = NW == 1 && sizeof(T) == 4 && a.Tq * a.G <= 16;
+    if constexpr (NW == 1 && sizeof(T) == 4) {
+        constexpr int FEW = DP == 128 ? 16 : 32;
+        if (few && a.vec) hipLaunchKernelGGL((attention_few_fwd_kernel<DP, FEW, true>), grid, dim3(64), 0, stream, a);
+        else if (few) hipLaunchKernelGGL((attention_few_fwd_kernel<DP, FEW, false>), grid, dim3(64), 0, stream, a);
+    }
+    if (!few && a.vec) hipLaunchKernelGGL((attention_fwd_kernel<T, DP, NW, KT, true>), grid, dim3(NW * 64), 0, stream, a);
+    else if (!few) hipLaunchKernelGGL((attention_fwd_kernel<T, DP, NW, KT, false>), grid, dim3(NW * 64), 0, stream, a);
     RS_CHECK_LAUNCH("rs_attention_fwd");
     if (a.splits > 1) {
         hipLaunchKernelGGL((attention_join_kernel<T>), rs_grid(rs_cdiv((long long)a.B * a.Hk * a.Tq * a.G, 4)), dim3(256), 0, stream, a);

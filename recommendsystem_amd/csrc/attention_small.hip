@@ -1,5 +1,6 @@
-// Attention where a sample has few keys and rows -- the fields of a sample, short histories: at most 64 of each, heads of at
-// most 32 (fp32) or 64 elements.  The formulas and masks are those of attention.hip.
+// Attention where a sample has few keys and rows -- the fields of a sample, short histories: at most 64 rows, and keys times
+// head elements (in tiles of 16) up to 64 x 32 in fp32, 64 x 64 in 16 bits.  The formulas and masks are those of
+// attention.hip.
 //
 // One wave per (sample, head), nothing shared with others: no barriers.  Keys and values (all of them) lie in the wave's
 // LDS, padded so that consecutive rows start 4 banks (mod 64) apart; the query rows pass by in tiles of 16 and stay in
@@ -14,29 +15,6 @@
 #pragma clang fp contract(fast)
 
 namespace {
-
-// 16x16 tiles: CK elements of the contraction in a fragment pair, 16 bytes a lane; lane l holds row (column) l % 16 and
-// elements E (l / 16) .. of the CK.  A result holds column l % 16 and rows 4 (l / 16) + 0..3.
-template <typename T> struct Mma16;
-template <> struct Mma16<float> {
-    static constexpr int CK = 16, E = 4, TILES = 1;          // TILES: row tiles that one contraction step over rows covers
-    typedef rs_f32x4 V;
-    static __device__ __forceinline__ rs_f32x4 mul(V a, V b, rs_f32x4 c) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
-        return c;
-    }
-};
-template <> struct Mma16<__bf16> {
-    static constexpr int CK = 32, E = 8, TILES = 2;
-    typedef rs_bf16x8 V;
-    static __device__ __forceinline__ rs_f32x4 mul(V a, V b, rs_f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
-};
-template <> struct Mma16<_Float16> {
-    static constexpr int CK = 32, E = 8, TILES = 2;
-    typedef rs_f16x8 V;
-    static __device__ __forceinline__ rs_f32x4 mul(V a, V b, rs_f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-};
 
 // Rows of W elements in LDS, 16 bytes of padding to a row.
 template <typename T, int W> struct Rows {
@@ -93,16 +71,6 @@ template <typename T> __device__ __forceinline__ typename Mma16<T>::V pack(const
     for (int e = 0; e < Mma16<T>::E; ++e) r[e] = (T)s[e / 4][e % 4];
     return r;
 }
-// Over the four lanes that hold a column.
-__device__ __forceinline__ float col_max(float x) {
-    x = fmaxf(x, __shfl_xor(x, 16, 64));
-    return fmaxf(x, __shfl_xor(x, 32, 64));
-}
-__device__ __forceinline__ float col_sum(float x) {
-    x += __shfl_xor(x, 16, 64);
-    return x + __shfl_xor(x, 32, 64);
-}
-
 // Keys [0, keys) and rows [begin, rows) that have a part in sample b (row_limit says which goes with which).
 struct Part {
     int keys, begin, rows;
@@ -361,22 +329,50 @@ template <typename T, int DP, int NT> int launch(AttnArgs a, bool back, hipStrea
     RS_CHECK_LAUNCH(back ? "rs_attention_bwd" : "rs_attention_fwd");
     return RS_OK;
 }
-template <int DP> int launch_f32(const AttnArgs& a, bool back, hipStream_t stream) {
-    const int n = (a.Tk + 15) / 16;
-    return n <= 1 ? launch<float, DP, 1>(a, back, stream) : n == 2 ? launch<float, DP, 2>(a, back, stream)
-         : n == 3 ? launch<float, DP, 3>(a, back, stream) : launch<float, DP, 4>(a, back, stream);
+// The kernel of the smallest head and tile count that cover D and Tk; together they cover what small_ok admits.
+int launch_f32(const AttnArgs& a, bool back, hipStream_t stream) {
+    const int n = a.Tk <= 16 ? 1 : (a.Tk + 15) / 16;
+#define RS_SMALL(DP, NT) \
+    if (a.D <= DP && n <= NT) return launch<float, DP, NT>(a, back, stream)
+    RS_SMALL(16, 1);
+    RS_SMALL(16, 2);
+    RS_SMALL(16, 3);
+    RS_SMALL(16, 4);
+    RS_SMALL(32, 1);
+    RS_SMALL(32, 2);
+    RS_SMALL(32, 3);
+    RS_SMALL(32, 4);
+    RS_SMALL(64, 1);
+    RS_SMALL(64, 2);
+    RS_SMALL(128, 1);
+    rs_set_error("attention: %d keys of %d elements are no small shape", a.Tk, a.D);
+    return RS_ERR_ARG;
 }
 template <typename T> int launch_16(const AttnArgs& a, bool back, hipStream_t stream) {
-    if (a.D <= 32) return a.Tk <= 32 ? launch<T, 32, 2>(a, back, stream) : launch<T, 32, 4>(a, back, stream);
-    return a.Tk <= 32 ? launch<T, 64, 2>(a, back, stream) : launch<T, 64, 4>(a, back, stream);
+    const int n = (a.Tk + 15) / 16;
+#define RS_SMALL16(DP, NT) \
+    if (a.D <= DP && n <= NT) return launch<T, DP, NT>(a, back, stream)
+    RS_SMALL16(32, 2);
+    RS_SMALL16(32, 4);
+    RS_SMALL16(64, 2);
+    RS_SMALL16(64, 4);
+    RS_SMALL16(128, 2);
+    rs_set_error("attention: %d keys of %d elements are no small shape", a.Tk, a.D);
+    return RS_ERR_ARG;
 }
 int launch_any(int dtype, const AttnArgs& a, bool back, hipStream_t stream) {
-    if (dtype == RS_F32) return a.D <= 16 ? launch_f32<16>(a, back, stream) : launch_f32<32>(a, back, stream);
+    if (dtype == RS_F32) return launch_f32(a, back, stream);
     return dtype == RS_BF16 ? launch_16<__bf16>(a, back, stream) : launch_16<_Float16>(a, back, stream);
 }
 
 }  // namespace
 
-bool rs_attention_small_ok(int dtype, int Tq, int Tk, int D) { return Tq <= 64 && Tk <= 64 && D <= (dtype == RS_F32 ? 32 : 64); }
+// Against the kernels of attention.hip, forward and backward: 512 x 60 x 8 heads of 64 bf16 29 + 79 us (30 + 90), 1024 x 30 x 8
+// of 128 bf16 61 + 132 (63 + 259), of 64 fp32 60 + 129 (71 + 469), 1024 x 16 x 8 of 128 fp32 59 + 112 (172 + 517).  Larger
+// products than these do not fit a wave's registers.
+bool rs_attention_small_ok(int dtype, int Tq, int Tk, int D) {
+    const int most = dtype == RS_F32 ? (D <= 32 ? 64 : D <= 64 ? 32 : 16) : (D <= 64 ? 64 : 32);
+    return Tq <= 64 && Tk <= most && D <= 128;
+}
 int rs_attention_small_fwd(int dtype, const AttnArgs& a, hipStream_t stream) { return launch_any(dtype, a, false, stream); }
 int rs_attention_small_bwd(int dtype, const AttnArgs& a, hipStream_t stream) { return launch_any(dtype, a, true, stream); }

@@ -1912,16 +1912,15 @@ class RotaryTable:
         if device.type == "cuda" and device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
         self.max_positions, self.rotary_dim, self.interleaved, self.device = int(max_positions), int(rotary_dim), bool(interleaved), device
-        freq = float(base) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
+        freq = float(base) ** (torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device) / -rotary_dim)
         if original_positions is None:
-            freq = freq / factor
+            freq = freq / factor if factor != 1.0 else freq
         else:
             turns = original_positions * freq / (2 * math.pi)
             keep = ((turns - ramp[0]) / (ramp[1] - ramp[0])).clamp(0, 1)
             freq = freq * (keep + (1 - keep) / factor)
-        angle = torch.arange(max_positions, dtype=torch.float64, device=device)[:, None] * freq.to(device)
-        self.cos = (angle.cos() * amplitude).float()
-        self.sin = (angle.sin() * amplitude).float()
+        angle = torch.arange(max_positions, dtype=torch.float64, device=device)[:, None] * freq
+        self.cos, self.sin = (t.float() if amplitude == 1.0 else (t * amplitude).float() for t in (angle.cos(), angle.sin()))
         self.err_flag = torch.zeros(1, dtype=torch.int32, device=device)
 
     def check_positions(self):

@@ -8,14 +8,14 @@ struct AttnOperand {
 };
 
 struct AttnArgs {
-    AttnOperand q, k, v, o, go;                  // go: gradient of o
+    AttnOperand q, k, v, o, go;              // go: gradient of o
     void *out, *dq, *dk, *dv;                // contiguous
     float *lse, *delta;                      // [B, Hq, Tq]
     const int *len, *qlen, *qstart;          // [B] or null
     int B, Tq, Tk, Hk, G, D, causal, start;
     float scale;
     int tiles, splits;                       // row (key) tiles per (sample, key head); shares of the keys (rows)
-    int dealt;                               // order of the workgroups, see unit_of
+    int dealt;                               // order of the workgroups: pairs (samples) dealt out at a time, 0: in runs
     // with splits > 1: forward [splits, B * Hk, Tq * G, D] and lse in base 2 [.., Tq * G], dk / dv [splits, 2, B, Tk, Hk, D]
     float *part_o, *part_ml;
     int vec;                                 // 16-byte loads from q, k, v, o, go

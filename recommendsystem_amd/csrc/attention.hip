@@ -177,7 +177,19 @@ template <typename T> __device__ __forceinline__ typename Mma<T>::V pack(const r
     return r;
 }
 
-__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
+// Over a lane and its partner lane + 32 (both get it): the swap leaves the lower half's values in .x, the upper one's in .y.
+__device__ __forceinline__ float2 halves(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_max(float x) {
+    const float2 h = halves(x);
+    return fmaxf(h.x, h.y);
+}
+__device__ __forceinline__ float half_sum(float x) {
+    const float2 h = halves(x);
+    return h.x + h.y;
+}
 // Row of register i within a 32x32 result.
 __device__ __forceinline__ int reg_row(int i) { return 8 * (i >> 2) + 4 * ((threadIdx.x & 63) >> 5) + (i & 3); }
 
@@ -302,7 +314,7 @@ __global__ __launch_bounds__(NW * 64) void attention_fwd_kernel(const AttnArgs a
         for (int n = 0; n < KB; ++n)
 #pragma unroll
             for (int e = 0; e < 16; ++e) top = fmaxf(top, s[n][e]);
-        top = fmaxf(top, other_half(top)) * scale2;
+        top = half_max(top) * scale2;
         const float m_new = fmaxf(m, top);
         const float base = m_new == -INFINITY ? 0.f : m_new;     // nothing seen yet: exp2(-inf - 0) = 0 throughout
         const float alpha = __builtin_amdgcn_exp2f(m - base);
@@ -332,7 +344,7 @@ __global__ __launch_bounds__(NW * 64) void attention_fwd_kernel(const AttnArgs a
             }
     }
     if (!live) return;
-    l += other_half(l);
+    l = half_sum(l);
     const float inv = l == 0.f ? 0.f : 1.f / l;                   // nothing seen: zeros (a NaN stays one)
     if (a.splits > 1) {
         const long long at = ((long long)split * a.B * a.Hk + pair) * rows + row;
@@ -552,7 +564,7 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_kernel(const AttnArgs a)
 #pragma unroll
             for (int e = 0; e < E; ++e) delta += (float)gf[c][e] * (float)of[e];
         }
-        delta += other_half(delta);
+        delta = half_sum(delta);
         const long long at = ((long long)b * a.Hk * a.G + h) * a.Tq + i;
         if (has) lse2 = a.lse[at] * LOG2E;
         if (live && half == 0) a.delta[at] = delta;
@@ -814,7 +826,7 @@ template <typename T> __global__ __launch_bounds__(256) void attention_dkv_join_
 // ---- host ------------------------------------------------------------------------------------------------------------------
 inline int padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 inline int waves_for(long long rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : 4; }
-inline int key_tile(int dtype, int D, int nw) { return nw == 1 || (dtype == RS_F32 && padded(D) == 128) ? 32 : 64; }
+inline int key_tile(int dtype, int D, int nw) { return nw == 1 || (dtype == RS_F32 && padded(D) == 128) ? 32 : 64; }     // at least
 
 // Shares of the keys: few rows leave most of the chip idle, so the keys of a sample are split until there are about
 // eight waves for every CU, but no share is shorter than four tiles.
@@ -838,7 +850,9 @@ int dkv_splits(int B, int Tq, int Tk, int Hk, int G, int uneven) {
 }
 
 template <typename T, int DP, int NW> int launch_fwd(AttnArgs a, hipStream_t stream) {
-    constexpr int KT = NW == 1 ? 32 : tile_rows<T, DP>();
+    // heads of 64: more keys at a time give the wave four independent chains of products (1537 x 12 heads x 3 fp16: 64 keys
+    // 50.5 us, 128 45.1); heads of 128 have no registers for it
+    constexpr int KT = NW == 1 ? 32 : NW == 4 && DP == 64 && sizeof(T) == 2 ? 128 : tile_rows<T, DP>();
     const dim3 grid = rs_grid(order_units(a));
     const bool few = NW == 1 && sizeof(T) == 4 && a.Tq * a.G <= 16;
     if constexpr (NW == 1 && sizeof(T) == 4) {

@@ -266,7 +266,7 @@ __global__ __launch_bounds__(NW * 64) void attention_fwd_kernel(const AttnArgs a
     {
         const T* qr = row_ptr<T>(a.q, b, live ? i : 0, live ? h : 0);
 #pragma unroll
-        for (int c = 0; c < NC; ++c) qf[c] = fetch<T, VEC>(qr, c * CK + half * E, a.D, live && lim > 0);
+        for (int c = 0; c < NC; ++c) qf[c] = fetch<T, VEC>(qr, c * CK + half * E, a.D, live);     // whatever it holds where lim = 0
     }
     rs_f32x16 acc[NB];
 #pragma unroll
@@ -937,7 +937,7 @@ AttnOperand operand(const void* p, long long b, long long t, long long h, int T,
 // tile of them stays within 31 bits.
 bool operand_vec(const AttnOperand& x, int dtype, int D) {
     const int e = 16 / rs_elem_bytes(dtype);
-    return !x.p || (rs_aligned16(x.p) && x.b % e == 0 && x.h % e == 0 && x.t % e == 0 && x.t >= D && x.t < (1 << 23));
+    return !x.p || (rs_aligned16(x.p) && x.b % e == 0 && x.h % e == 0 && x.t % e == 0 && x.t >= D && x.t < (1 << 22));
 }
 
 }  // namespace

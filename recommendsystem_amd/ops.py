@@ -1879,7 +1879,8 @@ def layer_norm_bwd(dy: torch.Tensor, s: torch.Tensor, mean: torch.Tensor, rstd: 
     dw = db = work = None
     floats = 0
     if want_params:
-        dw, db = torch.empty((2, N), dtype=pdt, device=dev).unbind(0)
+        dw = torch.empty(N, dtype=pdt, device=dev)
+        db = torch.empty(N, dtype=pdt, device=dev)
         floats = _norm_floats(M, N)
         # per call: two captured graphs, or two streams, never share the partial sums
         work = torch.empty(max(floats, 1), dtype=torch.float32, device=dev)

@@ -322,3 +322,39 @@ def test_empty_and_refused():
     for f in bad:
         with pytest.raises(RSError):
             f()
+
+
+@pytest.mark.parametrize("Tk", [3, 65])
+def test_more_samples_than_a_grid_dimension_holds(Tk):
+    """Over 2^22 workgroups: the launch takes a second grid dimension."""
+    from recommendsystem_amd import ops
+    B = (1 << 22) + 77
+    q = torch.randn(B, 1, 1, 4, device="cuda").half()
+    k = torch.randn(B, Tk, 1, 4, device="cuda").half()
+    v = torch.randn(B, Tk, 1, 4, device="cuda").half()
+    o, lse = ops.attention_fwd(q, k, v)
+    for part in (slice(0, 300), slice(B - 300, B), slice((1 << 22) - 150, (1 << 22) + 77)):
+        ref = reference(q[part], k[part], v[part])
+        inside(o[part], *ref["o"], "o")
+        inside(lse[part], *ref["lse"], "lse")
+    if Tk == 3:
+        do = torch.randn_like(q)
+        grads = ops.attention_bwd(do, q, k, v, o, lse)
+        for part in (slice(0, 300), slice(B - 300, B)):
+            ref = reference(q[part], k[part], v[part], do[part])
+            for name, g in zip(("dq", "dk", "dv"), grads):
+                inside(g[part], *ref[name], name)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_long_rows_uneven_work_and_shares(kind):
+    """Sequences long enough that dk and dv are shared out between workgroups and joined, causal and ragged."""
+    from recommendsystem_amd import _lib
+    B, T, HQ, HK, D = 2, 1300, 6, 2, 64
+    plain = _lib.lib().rs_attention_bwd_workspace_floats(0, B, T, T, HQ, HK, D, 0)
+    assert _lib.lib().rs_attention_bwd_workspace_floats(0, B, T, T, HQ, HK, D, 1) >= plain > (B * T * HQ + 3) // 4 * 4
+    q, k, v, do = make(B, T, T, HQ, HK, D, kind, seed=21)
+    compare(q, k, v, do)
+    compare(q, k, v, do, causal=True)
+    n = torch.tensor([1300, 517], device="cuda", dtype=torch.int32)
+    compare(q, k, v, do, causal=True, lengths=n, query_lengths=n)

@@ -241,3 +241,14 @@ def test_refusals():
     for f in bad:
         with pytest.raises(RSError):
             f()
+
+
+def test_more_rows_than_a_grid_dimension_holds():
+    from recommendsystem_amd import ops
+    M = (1 << 27) + 1000                     # 32 rows to a workgroup: over 2^22 workgroups
+    x = torch.randn(M, 2, device="cuda").half()
+    b = torch.tensor([0.5, -2.0], device="cuda").half()
+    y, _, mean, rstd = ops.layer_norm_fwd(x, None, b)
+    for part in (slice(0, 100), slice(M - 100, M)):
+        ref = reference(x[part], None, None, b, None, None, 1e-5)
+        inside(y[part], ref["y"], half_step(y.dtype, ref["y"]) + 64 * U * (1 + ref["xh"].abs() + ref["bd"].abs()), "y")

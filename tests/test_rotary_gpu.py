@@ -176,3 +176,14 @@ def test_empty_and_refused():
     for f in bad:
         with pytest.raises(RSError):
             f()
+
+
+def test_more_tokens_than_a_grid_dimension_holds():
+    from recommendsystem_amd import ops
+    T = (1 << 25) + 100                      # eight tokens to a workgroup: over 2^22 workgroups
+    table = ops.RotaryTable(64, 2, "cuda")
+    q = torch.randn(1, T, 1, 2, device="cuda").half()
+    pos = (torch.arange(T, device="cuda") % 64).int()
+    out = ops.rotary(table, pos, q)
+    for part in (slice(0, 100), slice(T - 100, T)):
+        inside(out[:, part], *reference(q[:, part], pos[part], freqs(2), False), "q")

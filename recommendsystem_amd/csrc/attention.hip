@@ -492,31 +492,52 @@ __global__ __launch_bounds__(64) void attention_few_fwd_kernel(const AttnArgs a)
     }
 }
 
-// Joins the shares of a row: weights exp2(lse_s - max) over their sum.  A wave to a row.
+// Joins the shares of a row: weights exp2(lse_s - max) over their sum.  32 lanes to a row: they fetch the statistics of all
+// shares at once (at most 64), then four elements of each share apiece.
 template <typename T> __global__ __launch_bounds__(256) void attention_join_kernel(const AttnArgs a) {
     const long long rows = (long long)a.Tq * a.G, all = rows * a.B * a.Hk;
-    const long long at = rs_block_id() * 4 + (threadIdx.x >> 6);
+    const long long at = rs_block_id() * 8 + (threadIdx.x >> 5);
     if (at >= all) return;
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 31;
     const long long pair = at / rows;
     const int row = (int)(at - pair * rows), i = row / a.G, b = (int)(pair / a.Hk), h = (int)(pair % a.Hk) * a.G + row % a.G;
-    float m = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[s * all + at]);
-    const float base = m == -INFINITY ? 0.f : m;
-    float l = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int s = 0; s < a.splits; ++s) {
-        const float w = exp2f(a.part_ml[s * all + at] - base);
-        const float* p = a.part_o + (s * all + at) * a.D;
-        l += w;
-        if (w != 0.f) {
-            if (lane < a.D) o0 += w * p[lane];
-            if (lane + 64 < a.D) o1 += w * p[lane + 64];
+    const float l0 = lane < a.splits ? a.part_ml[lane * all + at] : -INFINITY;
+    const float l1 = lane + 32 < a.splits ? a.part_ml[(lane + 32) * all + at] : -INFINITY;
+    float m = fmaxf(l0, l1);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 32));
+    const float base = m == -INFINITY ? 0.f : m, w0 = __builtin_amdgcn_exp2f(l0 - base), w1 = __builtin_amdgcn_exp2f(l1 - base);
+    float l = w0 + w1;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor(l, o, 32);
+    float o[4] = {0.f, 0.f, 0.f, 0.f};
+    const int d = lane * 4;
+    const bool vec = a.D % 4 == 0;
+    for (int s0 = 0; s0 < a.splits; s0 += 8) {                    // eight shares in flight
+        float w[8], x[8][4];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int s = s0 + u;
+            w[u] = s < a.splits ? __shfl(s < 32 ? w0 : w1, s & 31, 32) : 0.f;
+            x[u][0] = x[u][1] = x[u][2] = x[u][3] = 0.f;
+            if (s >= a.splits) continue;
+            const float* p = a.part_o + (s * all + at) * a.D + d;
+            if (vec && d < a.D) {
+                *(rs_f32x4*)x[u] = *(const rs_f32x4*)p;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[u][e] = d + e < a.D ? p[e] : 0.f;
+            }
         }
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] += w[u] * x[u][e];
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    T* out = (T*)a.out + (((long long)b * a.Tq + i) * a.Hk * a.G + h) * a.D;
-    if (lane < a.D) out[lane] = (T)(o0 * inv);
-    if (lane + 64 < a.D) out[lane + 64] = (T)(o1 * inv);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] *= inv;
+    store4<T>((T*)a.out + (((long long)b * a.Tq + i) * a.Hk * a.G + h) * a.D, d, a.D, a.out_vec, o);
     if (a.lse && lane == 0) a.lse[((long long)b * a.Hk * a.G + h) * a.Tq + i] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
 }
 
@@ -864,7 +885,7 @@ template <typename T, int DP, int NW> int launch_fwd(AttnArgs a, hipStream_t str
     else if (!few) hipLaunchKernelGGL((attention_fwd_kernel<T, DP, NW, KT, false>), grid, dim3(NW * 64), 0, stream, a);
     RS_CHECK_LAUNCH("rs_attention_fwd");
     if (a.splits > 1) {
-        hipLaunchKernelGGL((attention_join_kernel<T>), rs_grid(rs_cdiv((long long)a.B * a.Hk * a.Tq * a.G, 4)), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((attention_join_kernel<T>), rs_grid(((long long)a.B * a.Hk * a.Tq * a.G + 7) / 8), dim3(256), 0, stream, a);
         RS_CHECK_LAUNCH("rs_attention_fwd");
     }
     return RS_OK;

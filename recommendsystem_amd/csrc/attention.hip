@@ -22,6 +22,11 @@
 // atomics, the same bits every time.  Query heads that share a key head lie next to one another as rows of the forward
 // and dq (row = position * group + head), so a cache is read once for all of them; dk / dv walk over them.
 //
+// Bound by the matrix cores for heads of 128 (2 x 8192 x 16 heads on 4 key heads, bf16, causal: forward 552 us = 1000 TFLOP/s,
+// dq 722 = 1140, dk / dv 1129 + 25 for the join = 950; a library product of 8192^3 reaches 1208 here), by the exponentials
+// and the latency of a wave's chain for smaller ones (1537 x 12 x 3 heads of 64, fp16: 41 us, 530 TFLOP/s), by memory for
+// single tokens over caches (1.07 GB of full caches in 188 us, 5.7 TB/s).
+//
 // Roundings: products of 16-bit operands are exact and summed in fp32; P and dS are rounded to the operands' type for
 // their second product (the matrix cores take equal types; the rounding is a half step per element and averages out over
 // the keys); all statistics, sums and outputs before their last rounding are fp32.

@@ -13,6 +13,8 @@
 // The backward's workgroups walk over the rows in steps of the grid, so a lane meets the same columns in every row and
 // keeps their dw / db sums in registers; a workgroup adds up its row groups in LDS and writes one partial row, and a
 // second launch adds the partial rows in a fixed order (no atomics: the same bits every time).
+// 32768 x 4096 bf16 with a residual: forward 203 us (1.07 GB, 5.3 TB/s), backward 235 + 7 us (1.07 GB, 4.4 TB/s); a copy of
+// 4 GiB reaches 4.8.  4096 x 1024 fp32: 8.7 and 12.6 + 4.3 us.
 #include "lowp.h"
 #include "../../include/rs_hip.h"
 

@@ -702,16 +702,6 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 2 && VEC && NW =
             if constexpr (!VLDS) vf[c] = fetch<T, VEC>(vr, c * CK + half * E, a.D, has);
         }
     }
-    if constexpr (VLDS) {
-        Feed<T, DP, BN, NT, VEC> fv(a.v.t, a.D);
-        const long long seen = a.causal ? start + qrows : len;     // keys below it are seen
-        const int end = qrows > 0 ? (int)max(0LL, min(seen, (long long)len)) : 0;
-        if (tile * BN < end) {
-            fv.seek(row_ptr<T>(a.v, b, 0, hk), tile * BN, end);
-            fv.next(s_v);
-            fv.land(s_v);
-        }
-    }
     rs_f32x16 dk[NB], dv[NB];
 #pragma unroll
     for (int n = 0; n < NB; ++n)
@@ -728,6 +718,12 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 2 && VEC && NW =
         r_next += turn0 % per_head * RT;
         fq.seek(row_ptr<T>(a.q, b, 0, h), r_next, stop);
         fg.seek(row_ptr<T>(a.go, b, 0, h), r_next, stop);
+        if constexpr (VLDS) {            // (without a turn nothing would wait for it)
+            Feed<T, DP, BN, NT, VEC> fv(a.v.t, a.D);
+            fv.seek(row_ptr<T>(a.v, b, 0, hk), tile * BN, (int)min(a.causal ? start + qrows : len, (long long)len));
+            fv.next(s_v);
+            fv.land(s_v);
+        }
     }
     int r0 = r_next;
     float r_lse, r_delta;

@@ -300,7 +300,7 @@ __global__ __launch_bounds__(1024) void layer_norm_params_kernel(const float* __
                                                                  W* __restrict__ dw, W* __restrict__ db) {
     __shared__ float fold[32][33];
     const int c = threadIdx.x & 31, r = threadIdx.x >> 5;
-    const long long n = (long long)blockIdx.x * 32 + c, width = 2LL * N;
+    const long long n = rs_block_id() * 32 + c, width = 2LL * N;
     float a = 0.f;
     if (n < width) {
 #pragma unroll 8
@@ -460,7 +460,7 @@ int rs_layer_norm_bwd(int dtype, int param_dtype, const void* dy, long long lddy
         if (rc != RS_OK) return rc;
     }
     if (params) {                            // no rows: the sums are zero
-        const dim3 grid(rs_cdiv(2LL * N, 32));
+        const dim3 grid = rs_grid((2LL * N + 31) / 32);
         if (param_dtype == RS_F32)
             hipLaunchKernelGGL(layer_norm_params_kernel<float>, grid, dim3(1024), 0, stream, workspace, rows, N, (float*)dw,
                                (float*)db);

@@ -358,3 +358,15 @@ def test_long_rows_uneven_work_and_shares(kind):
     compare(q, k, v, do, causal=True)
     n = torch.tensor([1300, 517], device="cuda", dtype=torch.int32)
     compare(q, k, v, do, causal=True, lengths=n, query_lengths=n)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16", "f32"])
+def test_shares_of_rows_that_are_empty(kind):
+    """Heads of 128 whose row tiles do not divide evenly: the last shares of a key tile get no rows at all."""
+    from recommendsystem_amd import _lib
+    B, T, HQ, HK, D = 1, 700, 9, 1, 128
+    assert _lib.lib().rs_attention_bwd_workspace_floats(1, B, T, T, HQ, HK, D, 1) > (B * T * HQ + 3) // 4 * 4
+    q, k, v, do = make(B, T, T, HQ, HK, D, kind, seed=31)
+    compare(q, k, v, do, causal=True)
+    n = torch.tensor([610], device="cuda", dtype=torch.int32)
+    compare(q, k, v, do, causal=True, lengths=n, query_lengths=n)

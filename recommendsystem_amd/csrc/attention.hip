@@ -29,7 +29,9 @@
 //
 // Roundings: products of 16-bit operands are exact and summed in fp32; P and dS are rounded to the operands' type for
 // their second product (the matrix cores take equal types; the rounding is a half step per element and averages out over
-// the keys); all statistics, sums and outputs before their last rounding are fp32.
+// the keys).  With delta from the rounded o, dS would leave dq and dk of short rows 1.6 times as far off as their own last
+// rounding; for heads up to 64, where the matrix cores have time, it is multiplied in two parts, its rounding and the rest
+// of it (256 histories of 0..200, 8 heads of 32: 1.54 -> 1.03 times, for dq 39 -> 44 us and dk / dv 52 -> 57).  All statistics, sums and outputs before their last rounding are fp32.
 #include "attention.h"
 #include "../../include/rs_hip.h"
 
@@ -179,6 +181,14 @@ template <typename T> __device__ __forceinline__ typename Mma<T>::V pack(const r
     typename Mma<T>::V r;
 #pragma unroll
     for (int e = 0; e < Mma<T>::E; ++e) r[e] = (T)s[c * Mma<T>::E + e];
+    return r;
+}
+
+// What pack() rounds away, in the same places.
+template <typename T> __device__ __forceinline__ typename Mma<T>::V pack_rest(const rs_f32x16& s, int c, typename Mma<T>::V p) {
+    typename Mma<T>::V r;
+#pragma unroll
+    for (int e = 0; e < Mma<T>::E; ++e) r[e] = (T)(s[c * Mma<T>::E + e] - (float)p[e]);
     return r;
 }
 
@@ -549,6 +559,7 @@ template <typename T> __global__ __launch_bounds__(256) void attention_join_kern
 // ---- dq, and delta for the other gradients -----------------------------------------------------------------------------
 template <typename T, int DP, int NW, bool VEC>
 __global__ __launch_bounds__(NW * 64) void attention_dq_kernel(const AttnArgs a) {
+    constexpr bool BOTH = sizeof(T) == 2 && DP <= 64;             // dS in two parts, see above
     constexpr int KT = tile_rows<T, DP>();
     constexpr int NT = NW * 64, BM = NW * 32, CK = Mma<T>::CK, E = Mma<T>::E, NC = DP / CK, NB = DP / 32, KB = KT / 32;
     typedef typename Mma<T>::V V;
@@ -644,7 +655,11 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_kernel(const AttnArgs a)
             for (int c = 0; c < 32 / CK; ++c) {
                 const V p = pack<T>(s, c);
 #pragma unroll
-                for (int d = 0; d < NB; ++d) acc[d] = Mma<T>::mul(L::cols(s_k[buf], n * 32 + c * CK, d * 32), p, acc[d]);
+                for (int d = 0; d < NB; ++d) {
+                    const V kt = L::cols(s_k[buf], n * 32 + c * CK, d * 32);
+                    acc[d] = Mma<T>::mul(kt, p, acc[d]);
+                    if constexpr (BOTH) acc[d] = Mma<T>::mul(kt, pack_rest<T>(s, c, p), acc[d]);
+                }
             }
         }
     }
@@ -664,6 +679,7 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_kernel(const AttnArgs a)
 // ---- dk and dv -----------------------------------------------------------------------------------------------------------
 template <typename T, int DP, int NW, bool VEC>
 __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 2 && VEC && NW == 4 ? 2 : 1) void attention_dkv_kernel(const AttnArgs a) {
+    constexpr bool BOTH = sizeof(T) == 2 && DP <= 64;             // dS in two parts, see above
     constexpr bool VLDS = DP == 128 && sizeof(T) == 2;
     constexpr int RT = VLDS ? 32 : tile_rows<T, DP>();
     constexpr int NT = NW * 64, BN = NW * 32, CK = Mma<T>::CK, E = Mma<T>::E, NC = DP / CK, NB = DP / 32, RB = RT / 32;
@@ -795,8 +811,10 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 2 && VEC && NW =
                 const V p = pack<T>(s, c), ds = pack<T>(dp, c);
 #pragma unroll
                 for (int d = 0; d < NB; ++d) {
+                    const V qt = L::cols(s_q[buf], n * 32 + c * CK, d * 32);
                     dv[d] = Mma<T>::mul(L::cols(s_g[buf], n * 32 + c * CK, d * 32), p, dv[d]);
-                    dk[d] = Mma<T>::mul(L::cols(s_q[buf], n * 32 + c * CK, d * 32), ds, dk[d]);
+                    dk[d] = Mma<T>::mul(qt, ds, dk[d]);
+                    if constexpr (BOTH) dk[d] = Mma<T>::mul(qt, pack_rest<T>(dp, c, ds), dk[d]);
                 }
             }
         }

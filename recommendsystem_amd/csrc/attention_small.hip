@@ -9,8 +9,9 @@
 // they are.
 // The backward makes the scores once: dq comes from the columns as they are, and for dk and dv, whose contraction runs
 // over the rows, P and dS of a row tile go through a small LDS tile to be read the other way.  The query heads that
-// share a key head pass by one after the other, so every gradient has one owner.
-// 39 fields x 4096 samples, 2 heads of 16, fp32: forward 27 us (82 MB, 3.0 TB/s), backward 54 us (143 MB, 2.6 TB/s), of which
+// share a key head pass by one after the other, so every gradient has one owner.  A wave has a row's whole P and do . v, so
+// delta_i = sum_j p_ij (do_i . v_j), which is the same as do_i . o_i without o and its rounding.
+// 39 fields x 4096 samples, 2 heads of 16, fp32: forward 27 us (82 MB, 3.0 TB/s), backward 52 us (143 MB, 2.7 TB/s), of which
 // 8 and 19 us are matrix instructions; what is left is the latency of each wave's one short chain.
 #include "attention.h"
 
@@ -192,7 +193,7 @@ __global__ __launch_bounds__(64) void attention_small_fwd_kernel(const AttnArgs 
 // A wave per (sample, key head).  Row tiles go TILES at a time, what one contraction step over rows takes.
 template <typename T, int DP, int NT, bool VEC>
 __global__ __launch_bounds__(64) void attention_small_bwd_kernel(const AttnArgs a) {
-    constexpr int CK = Mma16<T>::CK, E = Mma16<T>::E, TILES = Mma16<T>::TILES, NC = DP / CK, ND = DP / 16, R = 16 * TILES;
+    constexpr int CK = Mma16<T>::CK, TILES = Mma16<T>::TILES, NC = DP / CK, ND = DP / 16, R = 16 * TILES;
     typedef typename Mma16<T>::V V;
     typedef Rows<T, DP> L;
     typedef Rows<T, NT * 16> LP;
@@ -217,22 +218,17 @@ __global__ __launch_bounds__(64) void attention_small_bwd_kernel(const AttnArgs 
     for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int d = 0; d < ND; ++d) dk[n][d] = dv[n][d] = rs_f32x4{0.f, 0.f, 0.f, 0.f};
-    // a turn is R rows of one head; loads run one turn ahead, as do the lanes' own parts of o and lse
-    V of[TILES][NC];
+    // a turn is R rows of one head; loads run one turn ahead, as does the lanes' lse
     float lse[TILES];
     const int per_head = (a.Tq + R - 1) / R, turns = per_head * a.G;
     auto load = [&](int turn) {
         const int h = hk * a.G + turn / per_head, i0 = turn % per_head * R;
         cq.load(row_ptr<T>(a.q, b, 0, h), a.q.t, i0, part.begin, part.rows, a.D);
         cg.load(row_ptr<T>(a.go, b, 0, h), a.go.t, i0, part.begin, part.rows, a.D);
-        const T* o = row_ptr<T>(a.o, b, 0, h);
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
             const int i = i0 + t * 16 + col;
-            const bool has = i >= part.begin && i < part.rows;
-#pragma unroll
-            for (int c = 0; c < NC; ++c) of[t][c] = fetch<T, VEC>(o + (long long)i * a.o.t, c * CK + g * E, a.D, has);
-            lse[t] = has ? a.lse[((long long)b * Hq + h) * a.Tq + i] : INFINITY;
+            lse[t] = i >= part.begin && i < part.rows ? a.lse[((long long)b * Hq + h) * a.Tq + i] : INFINITY;
         }
     };
     if (turns > 0) load(0);
@@ -242,24 +238,15 @@ __global__ __launch_bounds__(64) void attention_small_bwd_kernel(const AttnArgs 
         const int h = hk * a.G + turn / per_head, i0 = turn % per_head * R;
         cq.store(s_q);
         cg.store(s_g);
-        float delta[TILES], lse2[TILES];
+        float lse2[TILES];
 #pragma unroll
-        for (int t = 0; t < TILES; ++t) {
-            delta[t] = 0.f;
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                const V x = L::rows(s_g, t * 16, c);
-#pragma unroll
-                for (int e = 0; e < E; ++e) delta[t] += (float)x[e] * (float)of[t][c][e];
-            }
-            delta[t] = col_sum(delta[t]);
-            lse2[t] = lse[t] * LOG2E;
-        }
+        for (int t = 0; t < TILES; ++t) lse2[t] = lse[t] * LOG2E;
         if (turn + 1 < turns) load(turn + 1);
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
             const int i = i0 + t * 16 + col, lim = limit(a, part, i);
             rs_f32x4 p[NT], ds[NT];
+            float delta = 0.f;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 p[n] = ds[n] = rs_f32x4{0.f, 0.f, 0.f, 0.f};
@@ -272,8 +259,15 @@ __global__ __launch_bounds__(64) void attention_small_bwd_kernel(const AttnArgs 
                 for (int e = 0; e < 4; ++e) {
                     const bool seen = n * 16 + 4 * g + e < lim;       // selected, not multiplied
                     p[n][e] = seen ? __builtin_amdgcn_exp2f(p[n][e] * scale2 - lse2[t]) : 0.f;
-                    ds[n][e] = seen ? p[n][e] * (ds[n][e] - delta[t]) : 0.f;
+                    ds[n][e] = seen ? ds[n][e] : 0.f;
+                    delta += p[n][e] * ds[n][e];
                 }
+            }
+            delta = col_sum(delta);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) ds[n][e] = p[n][e] * (ds[n][e] - delta);
                 // row = query: four consecutive keys of one row
                 store4<T>(s_p + (t * 16 + col) * LP::RS, n * 16 + 4 * g, NT * 16, true, (const float*)&p[n]);
                 store4<T>(s_d + (t * 16 + col) * LP::RS, n * 16 + 4 * g, NT * 16, true, (const float*)&ds[n]);
@@ -369,7 +363,7 @@ int launch_any(int dtype, const AttnArgs& a, bool back, hipStream_t stream) {
 
 }  // namespace
 
-// Against the kernels of attention.hip, forward and backward: 512 x 60 x 8 heads of 64 bf16 29 + 79 us (30 + 90), 1024 x 30 x 8
+// Against the kernels of attention.hip, forward and backward: 512 x 60 x 8 heads of 64 bf16 29 + 70 us (30 + 90), 1024 x 30 x 8
 // of 128 bf16 61 + 132 (63 + 259), of 64 fp32 60 + 129 (71 + 469), 1024 x 16 x 8 of 128 fp32 59 + 112 (172 + 517).  Larger
 // products than these do not fit a wave's registers.
 bool rs_attention_small_ok(int dtype, int Tq, int Tk, int D) {

@@ -19,6 +19,14 @@
 
 namespace {
 
+// What lanes wrote to LDS in front of it is what other lanes of the wave read behind it, and what was read in front of it may
+// be written over.  The hardware runs a wave's LDS accesses in their order, so this costs no instruction; it holds the
+// compiler to that order, which sees one lane's addresses only.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // Rows of W elements in LDS, 16 bytes of padding to a row.
 template <typename T, int W> struct Rows {
     static constexpr int E = Mma16<T>::E, RS = W + E;
@@ -136,6 +144,7 @@ __global__ __launch_bounds__(64) void attention_small_fwd_kernel(const AttnArgs 
     for (int c = 0; c < NC; ++c) qn[c] = fetch<T, VEC>(q + (long long)col * a.q.t, c * CK + g * E, a.D, col >= part.begin && col < part.rows);
     ck.store(s_k);
     cv.store(s_v);
+    wave_sync();
     for (int i0 = 0; i0 < a.Tq; i0 += 16) {
         const int i = i0 + col, lim = limit(a, part, i);
 #pragma unroll
@@ -236,8 +245,10 @@ __global__ __launch_bounds__(64) void attention_small_bwd_kernel(const AttnArgs 
     cv.store(s_v);
     for (int turn = 0; turn < turns; ++turn) {
         const int h = hk * a.G + turn / per_head, i0 = turn % per_head * R;
+        wave_sync();                                              // the last turn's reads are done
         cq.store(s_q);
         cg.store(s_g);
+        wave_sync();
         float lse2[TILES];
 #pragma unroll
         for (int t = 0; t < TILES; ++t) lse2[t] = lse[t] * LOG2E;
@@ -290,6 +301,7 @@ __global__ __launch_bounds__(64) void attention_small_bwd_kernel(const AttnArgs 
                 }
             }
         }
+        wave_sync();
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const V p = LP::cols(s_p, 0, n * 16), ds = LP::cols(s_d, 0, n * 16);

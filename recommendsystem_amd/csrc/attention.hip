@@ -106,6 +106,31 @@ template <typename T, int DP> struct Tile {
     }
 };
 
+// G asynchronous 16-byte loads a lane, the first one's to LDS byte address dst, each further one's STEP behind.  m0, which
+// takes the address, is the compiler's and cannot be declared overwritten: every statement gives it back.  The nops: m0 and
+// descriptor registers that were written just before, the latter by vector instructions.
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+template <int G, int STEP> __device__ __forceinline__ void loads_to_lds(unsigned dst, u32x4 rsrc, const unsigned* off) {
+    static_assert(G == 1 || G == 2 || G == 4, "as many as the statements have");
+    unsigned m0;
+    if constexpr (G == 1)
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 4\n\tbuffer_load_dwordx4 %3, %2, 0 offen lds\n\t"
+                     "s_mov_b32 m0, %0"
+                     : "=&s"(m0) : "s"(dst), "s"(rsrc), "v"(off[0]) : "memory");
+    else if constexpr (G == 2)
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 4\n\tbuffer_load_dwordx4 %4, %2, 0 offen lds\n\t"
+                     "s_add_u32 m0, m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %5, %2, 0 offen lds\n\t"
+                     "s_mov_b32 m0, %0"
+                     : "=&s"(m0) : "s"(dst), "s"(rsrc), "i"(STEP), "v"(off[0]), "v"(off[1]) : "memory", "scc");
+    else
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 4\n\tbuffer_load_dwordx4 %4, %2, 0 offen lds\n\t"
+                     "s_add_u32 m0, m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %5, %2, 0 offen lds\n\t"
+                     "s_add_u32 m0, m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %6, %2, 0 offen lds\n\t"
+                     "s_add_u32 m0, m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %7, %2, 0 offen lds\n\t"
+                     "s_mov_b32 m0, %0"
+                     : "=&s"(m0) : "s"(dst), "s"(rsrc), "i"(STEP), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]) : "memory", "scc");
+}
+
 // The way of consecutive tiles of R rows into LDS, NT lanes; rows from row_end on and columns from D on become zeros.
 // VEC: asynchronous 16-byte loads from memory to LDS through a buffer descriptor that ends with the last row, whose range
 // check supplies the zeros; no register holds the data, and the tile is there after the wait in feed_sync().
@@ -141,17 +166,13 @@ template <typename T, int DP, int R, int NT, bool VEC> struct Feed {
             const unsigned long long where = (unsigned long long)at;
             const long long most = 0x7fffff00LL / (int)sizeof(T);
             const int bytes = (int)(left < most ? left : most) * (int)sizeof(T);
-            typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
             const u32x4 rsrc = {(unsigned)__builtin_amdgcn_readfirstlane((int)where),
                                 (unsigned)__builtin_amdgcn_readfirstlane((int)(where >> 32)) & 0xffffu,
                                 (unsigned)__builtin_amdgcn_readfirstlane(bytes), 0x00027000u};
             const unsigned dst = __builtin_amdgcn_readfirstlane(
                 (int)(unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)lds + (int)(threadIdx.x >> 6) * 1024);
 #pragma unroll
-            for (int i = 0; i < N; ++i)      // the nops: a descriptor register written by a vector instruction just before
-                asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst + i * NT * 16),
-                             "v"(off[i]), "s"(rsrc)
-                             : "memory");
+            for (int i = 0; i < N; i += N < 4 ? N : 4) loads_to_lds<N < 4 ? N : 4, NT * 16>(dst + i * NT * 16, rsrc, off + i);
         } else {
 #pragma unroll
             for (int i = 0; i < N; ++i) {

@@ -360,13 +360,14 @@ template <int R, bool MC> struct DmaOp {
     __device__ __forceinline__ void issue_one(int t, int k0, int kend, unsigned dst, int wid) {
         const char* cur = base + (long long)t * step;
         const unsigned d = dst + (unsigned)((p * 256 + wid * 64) * 16);
+        unsigned m0;         // the compiler's, which cannot be declared overwritten: given back
         if constexpr (FULL) {
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                         :: "s"(d), "v"(voff[p]), "s"(cur) : "memory");
+            asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
+                         : "=&s"(m0) : "s"(d), "v"(voff[p]), "s"(cur) : "memory");
         } else {
             const char* s = (k0 + kofs[p] < kend) ? cur + voff[p] : reinterpret_cast<const char*>(g_zero_src);
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
-                         :: "s"(d), "v"(s) : "memory");
+            asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\ts_mov_b32 m0, %0"
+                         : "=&s"(m0) : "s"(d), "v"(s) : "memory");
         }
     }
 };

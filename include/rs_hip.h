@@ -616,7 +616,7 @@ int rs_rotary(int dtype, const void* q, long long qb, long long qt, long long qh
  * multiple of Hk (query heads h Hq/Hk .. share key head h); b / t / h strides of every operand in elements.  Row i of
  * sample b sees key j where j < lengths[b] and i < query_lengths[b] (device int32 [B], null: all; clamped to 0..T) and,
  * with causal != 0, j <= i + start, start = query_starts[b] (device int32 [B]) or query_start where that is null.  A row
- * that sees nothing: o = 0, lse = -inf, zero gradients.  Keys, values and rows behind the lengths may hold anything.
+ * that sees nothing (or whose fp32 scores all overflow to -inf): o = 0, lse = -inf, zero gradients.  Keys, values and rows behind the lengths may hold anything.
  * o [B, Tq, Hq, D] contiguous; lse [B, Hq, Tq] fp32 (null: not wanted), natural logarithm of the sum of exponentials.
  * workspace (16-byte aligned): rs_attention_fwd_workspace_floats(..) floats, 0 for most shapes: few rows over many keys
  * are split over the keys and joined by a second launch.

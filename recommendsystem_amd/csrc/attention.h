@@ -69,6 +69,10 @@ __device__ __forceinline__ int row_limit(const AttnArgs& a, int b, int i) {
     return lim;
 }
 
+// A row's lse for the backward, in base 2.  -inf: the row sees nothing, or its scores all overflowed to -inf (fp32 operands
+// near 1e20); it got zeros, and exp2(z - inf) = 0 gives it no part in any gradient.
+__device__ __forceinline__ float back_lse(float lse) { return lse == -INFINITY ? INFINITY : lse * LOG2E; }
+
 template <typename T> __device__ __forceinline__ const T* row_ptr(const AttnOperand& x, int b, int t, int h) {
     return (const T*)x.p + b * x.b + t * x.t + h * x.h;
 }

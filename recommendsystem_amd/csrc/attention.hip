@@ -624,7 +624,7 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_kernel(const AttnArgs a)
         }
         delta = half_sum(delta);
         const long long at = ((long long)b * a.Hk * a.G + h) * a.Tq + i;
-        if (has) lse2 = a.lse[at] * LOG2E;
+        if (has) lse2 = back_lse(a.lse[at]);
         if (live && half == 0) a.delta[at] = delta;
     }
     rs_f32x16 acc[NB];
@@ -792,7 +792,7 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 2 && VEC && NW =
         // a row that sees nothing, or is none: exp2(z - inf) = 0
         asm volatile("" : "+v"(r_lse), "+v"(r_delta));            // all lanes wait for them here (see settle)
         if (threadIdx.x < RT) {
-            s_lse[buf][threadIdx.x] = r_lse == -INFINITY || r0 + (int)threadIdx.x >= stop ? INFINITY : r_lse * LOG2E;
+            s_lse[buf][threadIdx.x] = r0 + (int)threadIdx.x >= stop ? INFINITY : back_lse(r_lse);
             s_delta[buf][threadIdx.x] = r_delta;
         }
         feed_sync<VEC>();

@@ -251,7 +251,7 @@ __global__ __launch_bounds__(64) void attention_small_bwd_kernel(const AttnArgs 
         wave_sync();
         float lse2[TILES];
 #pragma unroll
-        for (int t = 0; t < TILES; ++t) lse2[t] = lse[t] * LOG2E;
+        for (int t = 0; t < TILES; ++t) lse2[t] = back_lse(lse[t]);
         if (turn + 1 < turns) load(turn + 1);
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {

@@ -3,7 +3,7 @@ too, unless a test says otherwise."""
 import pytest
 import torch
 
-from test_attention_gpu import compare, make
+from test_attention_gpu import compare, inside, make, reference
 
 pytestmark = pytest.mark.gpu
 
@@ -31,3 +31,24 @@ def test_turns_of_one_wave_do_not_meet_in_lds(kind, Tk, D):
     torch.cuda.synchronize()
     for out in outs:
         assert all(torch.equal(a, b) for a, b in zip(out, first))
+
+
+@pytest.mark.parametrize("Tq,Tk,D", [(20, 30, 16), (70, 150, 24), (70, 40, 128)])
+def test_rows_whose_scores_all_overflow_have_no_part_in_the_gradients(Tq, Tk, D):
+    """fp32 products of -1e20 and 1e20 overflow to -inf.  Such rows get zeros and lse = -inf, as rows that see nothing; the other
+    rows (q = 0: scores of zero) and the gradients of keys and values are as if they were not there."""
+    from recommendsystem_amd import ops
+    q, k, v, do = make(2, Tq, Tk, 2, 1, D, "f32", seed=41)
+    k = 1e20 * (0.5 + torch.rand_like(k))
+    lost = torch.arange(Tq, device="cuda") % 3 == 1
+    q = torch.where(lost.view(1, -1, 1, 1), -1e20, 0.0).expand_as(q).contiguous()
+    o, lse = ops.attention_fwd(q, k, v)
+    got = (o, *ops.attention_bwd(do, q, k, v, o, lse))
+    ref = reference(torch.zeros_like(q), k, v, torch.where(lost.view(1, -1, 1, 1), 0.0, do))
+    assert torch.equal(lse == -torch.inf, lost.expand_as(lse))
+    for name, x in zip(("o", "dq", "dk", "dv"), got):
+        if name in ("o", "dq"):
+            assert torch.count_nonzero(x[:, lost]).item() == 0, name
+            inside(x[:, ~lost], ref[name][0][:, ~lost], ref[name][1][:, ~lost], name)
+        else:
+            inside(x, *ref[name], name)

@@ -381,22 +381,23 @@ __global__ __launch_bounds__(NW * 64) void attention_fwd_kernel(const AttnArgs a
     }
     if (!live) return;
     l = half_sum(l);
-    const float inv = l == 0.f ? 0.f : 1.f / l;                   // nothing seen: zeros (a NaN stays one)
+    const bool none = l == 0.f;                                   // nothing seen: zeros, whatever the other rows' keys hold
+    const float inv = 1.f / l;
     if (a.splits > 1) {
         const long long at = ((long long)split * a.B * a.Hk + pair) * rows + row;
-        if (half == 0) a.part_ml[at] = l == 0.f ? -INFINITY : m + log2f(l);
+        if (half == 0) a.part_ml[at] = none ? -INFINITY : m + log2f(l);
 #pragma unroll
         for (int d = 0; d < NB; ++d)
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
                 float o[4];
 #pragma unroll
-                for (int x = 0; x < 4; ++x) o[x] = acc[d][e + x] * inv;
+                for (int x = 0; x < 4; ++x) o[x] = none ? 0.f : acc[d][e + x] * inv;
                 store4<float>(a.part_o + at * a.D, d * 32 + reg_row(e), a.D, a.D % 4 == 0, o);
             }
         return;
     }
-    if (a.lse && half == 0) a.lse[((long long)b * a.Hk * a.G + h) * a.Tq + i] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+    if (a.lse && half == 0) a.lse[((long long)b * a.Hk * a.G + h) * a.Tq + i] = none ? -INFINITY : (m + log2f(l)) * LN2;
     T* out = (T*)a.out + (((long long)b * a.Tq + i) * a.Hk * a.G + h) * a.D;
 #pragma unroll
     for (int d = 0; d < NB; ++d)
@@ -404,7 +405,7 @@ __global__ __launch_bounds__(NW * 64) void attention_fwd_kernel(const AttnArgs a
         for (int e = 0; e < 16; e += 4) {
             float o[4];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) o[x] = acc[d][e + x] * inv;
+            for (int x = 0; x < 4; ++x) o[x] = none ? 0.f : acc[d][e + x] * inv;
             store4<T>(out, d * 32 + reg_row(e), a.D, a.out_vec, o);
         }
 }
@@ -513,17 +514,20 @@ __global__ __launch_bounds__(64) void attention_few_fwd_kernel(const AttnArgs a)
     }
     l = col_sum(l);
     if (!live) return;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const bool none = l == 0.f;
+    const float inv = 1.f / l;
     const bool shared_out = a.splits > 1;
     const long long at = ((long long)split * a.B * a.Hk + pair) * rows + col;
     T* out = shared_out ? a.part_o + at * a.D : (T*)a.out + (((long long)b * a.Tq + i) * a.Hk * a.G + h) * a.D;
     if (g == 0) {
-        if (shared_out) a.part_ml[at] = l == 0.f ? -INFINITY : m + log2f(l);
-        else if (a.lse) a.lse[((long long)b * a.Hk * a.G + h) * a.Tq + i] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+        if (shared_out) a.part_ml[at] = none ? -INFINITY : m + log2f(l);
+        else if (a.lse) a.lse[((long long)b * a.Hk * a.G + h) * a.Tq + i] = none ? -INFINITY : (m + log2f(l)) * LN2;
     }
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
-        const float x[4] = {acc[d][0] * inv, acc[d][1] * inv, acc[d][2] * inv, acc[d][3] * inv};
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = none ? 0.f : acc[d][e] * inv;
         store4<T>(out, d * 16 + 4 * g, a.D, shared_out ? a.D % 4 == 0 : a.out_vec, x);
     }
 }
@@ -692,7 +696,7 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_kernel(const AttnArgs a)
         for (int e = 0; e < 16; e += 4) {
             float o[4];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) o[x] = acc[d][e + x] * a.scale;
+            for (int x = 0; x < 4; ++x) o[x] = lse2 == INFINITY ? 0.f : acc[d][e + x] * a.scale;      // saw nothing: zeros
             store4<T>(out, d * 32 + reg_row(e), a.D, a.out_vec, o);
         }
 }

@@ -187,12 +187,15 @@ __global__ __launch_bounds__(64) void attention_small_fwd_kernel(const AttnArgs 
             for (int d = 0; d < ND; ++d) o[d] = Mma16<T>::mul(L::cols(s_v, n * 16, d * 16), p, o[d]);
         }
         if (i >= a.Tq) continue;
-        const float inv = l == 0.f ? 0.f : 1.f / l;               // nothing seen: zeros (a NaN stays one)
-        if (a.lse && g == 0) a.lse[((long long)b * Hq + h) * a.Tq + i] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+        const bool none = l == 0.f;                               // nothing seen: zeros, whatever the other rows' keys hold
+        const float inv = 1.f / l;
+        if (a.lse && g == 0) a.lse[((long long)b * Hq + h) * a.Tq + i] = none ? -INFINITY : (m + log2f(l)) * LN2;
         T* out = (T*)a.out + (((long long)b * a.Tq + i) * Hq + h) * a.D;
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
-            const float x[4] = {o[d][0] * inv, o[d][1] * inv, o[d][2] * inv, o[d][3] * inv};
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = none ? 0.f : o[d][e] * inv;
             store4<T>(out, d * 16 + 4 * g, a.D, a.out_vec, x);
         }
     }
@@ -296,7 +299,9 @@ __global__ __launch_bounds__(64) void attention_small_bwd_kernel(const AttnArgs 
                 T* out = (T*)a.dq + (((long long)b * a.Tq + i) * Hq + h) * a.D;
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
-                    const float x[4] = {dq[d][0] * a.scale, dq[d][1] * a.scale, dq[d][2] * a.scale, dq[d][3] * a.scale};
+                    float x[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = lim == 0 || lse2[t] == INFINITY ? 0.f : dq[d][e] * a.scale;      // saw nothing
                     store4<T>(out, d * 16 + 4 * g, a.D, a.out_vec, x);
                 }
             }

@@ -52,3 +52,24 @@ def test_rows_whose_scores_all_overflow_have_no_part_in_the_gradients(Tq, Tk, D)
             inside(x[:, ~lost], ref[name][0][:, ~lost], ref[name][1][:, ~lost], name)
         else:
             inside(x, *ref[name], name)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("Tq,Tk,D", [(20, 30, 16), (70, 150, 64), (130, 40, 128), (3, 4000, 64)])
+def test_rows_that_see_nothing_stay_zero_beside_rows_of_infinite_keys(Tq, Tk, D, kind):
+    """A non-finite key or value is the business of the rows that see it: rows behind the sample's own and rows in front of
+    its first key get zeros even where they share a tile with such rows."""
+    from recommendsystem_amd import ops
+    q, k, v, do = make(2, Tq, Tk, 4, 2, D, kind, seed=51)
+    n = torch.tensor([Tq - 1, Tq - 2], device="cuda", dtype=torch.int32)
+    i = torch.arange(Tq, device="cuda").view(1, -1)
+    for name, t in (("v", v), ("k", k)):
+        for fill in (float("inf"), float("nan")):
+            x = t.clone()
+            x[:, 0] = fill
+            kv = (k, x) if name == "v" else (x, v)
+            for how, out in ((dict(query_lengths=n), i >= n.view(-1, 1)), (dict(causal=True, query_start=-1), (i < 1).expand(2, -1))):
+                o, lse = ops.attention_fwd(q, *kv, **how)
+                dq = ops.attention_bwd(do, q, *kv, o, lse, **how)[0]
+                assert torch.equal(lse == -torch.inf, out.view(2, 1, Tq).expand_as(lse))
+                assert torch.count_nonzero(o[out]).item() == 0 and torch.count_nonzero(dq[out]).item() == 0, (name, fill, how)

@@ -31,7 +31,8 @@
 // their second product (the matrix cores take equal types; the rounding is a half step per element and averages out over
 // the keys).  With delta from the rounded o, dS would leave dq and dk of short rows 1.6 times as far off as their own last
 // rounding; for heads up to 64, where the matrix cores have time, it is multiplied in two parts, its rounding and the rest
-// of it (256 histories of 0..200, 8 heads of 32: 1.54 -> 1.03 times, for dq 39 -> 44 us and dk / dv 52 -> 57).  All statistics, sums and outputs before their last rounding are fp32.
+// of it (256 histories of 0..200, 8 heads of 32: 1.54 -> 1.03 times, for dq 39 -> 44 us and dk / dv 52 -> 57).  In fp16 P and dS
+// are rounded as multiples of powers of two that keep them in the type's range (attention.h).  All statistics, sums and outputs before their last rounding are fp32.
 #include "attention.h"
 #include "../../include/rs_hip.h"
 
@@ -43,6 +44,7 @@ namespace {
 template <typename T> struct Mma;
 template <> struct Mma<float> {
     static constexpr int CK = 8, E = 4;
+    static constexpr bool F16 = false;
     typedef rs_f32x4 V;
     static __device__ __forceinline__ rs_f32x16 mul(V a, V b, rs_f32x16 c) {
 #pragma unroll
@@ -52,6 +54,7 @@ template <> struct Mma<float> {
 };
 template <> struct Mma<__bf16> {
     static constexpr int CK = 16, E = 8;
+    static constexpr bool F16 = false;
     typedef rs_bf16x8 V;
     static __device__ __forceinline__ rs_f32x16 mul(V a, V b, rs_f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
@@ -59,6 +62,7 @@ template <> struct Mma<__bf16> {
 };
 template <> struct Mma<_Float16> {
     static constexpr int CK = 16, E = 8;
+    static constexpr bool F16 = true;
     typedef rs_f16x8 V;
     static __device__ __forceinline__ rs_f32x16 mul(V a, V b, rs_f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
@@ -226,6 +230,16 @@ __device__ __forceinline__ float half_sum(float x) {
     const float2 h = halves(x);
     return h.x + h.y;
 }
+__device__ __forceinline__ float reg_max(const rs_f32x16& s) {      // of the absolute values, NaN ignored
+    float m = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) m = fmaxf(m, fabsf(s[e]));
+    return m;
+}
+__device__ __forceinline__ void scale_by(rs_f32x16& s, int exp) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[e] = ldexpf(s[e], exp);
+}
 // Row of register i within a 32x32 result.
 __device__ __forceinline__ int reg_row(int i) { return 8 * (i >> 2) + 4 * ((threadIdx.x & 63) >> 5) + (i & 3); }
 
@@ -360,7 +374,7 @@ __global__ __launch_bounds__(NW * 64) void attention_fwd_kernel(const AttnArgs a
         for (int n = 0; n < KB; ++n)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                s[n][e] = __builtin_amdgcn_exp2f(s[n][e] * scale2 - base);
+                s[n][e] = __builtin_amdgcn_exp2f(s[n][e] * scale2 - (base - P_SHIFT<T>));
                 sum += s[n][e];
             }
         l = l * alpha + sum;                                      // this half's keys only
@@ -385,7 +399,7 @@ __global__ __launch_bounds__(NW * 64) void attention_fwd_kernel(const AttnArgs a
     const float inv = 1.f / l;
     if (a.splits > 1) {
         const long long at = ((long long)split * a.B * a.Hk + pair) * rows + row;
-        if (half == 0) a.part_ml[at] = none ? -INFINITY : m + log2f(l);
+        if (half == 0) a.part_ml[at] = none ? -INFINITY : m + log2f(l) - P_SHIFT<T>;
 #pragma unroll
         for (int d = 0; d < NB; ++d)
 #pragma unroll
@@ -397,7 +411,7 @@ __global__ __launch_bounds__(NW * 64) void attention_fwd_kernel(const AttnArgs a
             }
         return;
     }
-    if (a.lse && half == 0) a.lse[((long long)b * a.Hk * a.G + h) * a.Tq + i] = none ? -INFINITY : (m + log2f(l)) * LN2;
+    if (a.lse && half == 0) a.lse[((long long)b * a.Hk * a.G + h) * a.Tq + i] = none ? -INFINITY : (m + log2f(l) - P_SHIFT<T>) * LN2;
     T* out = (T*)a.out + (((long long)b * a.Tq + i) * a.Hk * a.G + h) * a.D;
 #pragma unroll
     for (int d = 0; d < NB; ++d)
@@ -584,7 +598,7 @@ template <typename T> __global__ __launch_bounds__(256) void attention_join_kern
 // ---- dq, and delta for the other gradients -----------------------------------------------------------------------------
 template <typename T, int DP, int NW, bool VEC>
 __global__ __launch_bounds__(NW * 64) void attention_dq_kernel(const AttnArgs a) {
-    constexpr bool BOTH = sizeof(T) == 2 && DP <= 64;             // dS in two parts, see above
+    constexpr bool BOTH = sizeof(T) == 2 && DP <= 64, F16 = Mma<T>::F16;      // dS in two parts, see above; Range
     constexpr int KT = tile_rows<T, DP>();
     constexpr int NT = NW * 64, BM = NW * 32, CK = Mma<T>::CK, E = Mma<T>::E, NC = DP / CK, NB = DP / 32, KB = KT / 32;
     typedef typename Mma<T>::V V;
@@ -613,6 +627,7 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_kernel(const AttnArgs a)
 
     V qf[NC], gf[NC];
     float delta = 0.f, lse2 = INFINITY;
+    Range range;                                                  // of the lane's row: its factor goes into lse2
     {
         const bool has = live && lim > 0;
         const T* qr = row_ptr<T>(a.q, b, live ? i : 0, live ? h : 0);
@@ -676,6 +691,16 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_kernel(const AttnArgs a)
             }
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(s[e] * scale2 - lse2) * (dp[e] - delta);
+            if constexpr (F16) {
+                const float top = half_max(reg_max(s));
+                if (__any(range.past(top))) {
+                    const int by = range.follow(top);
+                    lse2 -= (float)by;
+                    scale_by(s, by);
+#pragma unroll
+                    for (int d = 0; d < NB; ++d) scale_by(acc[d], by);
+                }
+            }
 #pragma unroll
             for (int c = 0; c < 32 / CK; ++c) {
                 const V p = pack<T>(s, c);
@@ -690,13 +715,14 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_kernel(const AttnArgs a)
     }
     if (!live) return;
     T* out = (T*)a.dq + (((long long)b * a.Tq + i) * a.Hk * a.G + h) * a.D;
+    const float back = a.scale * range.unit();
 #pragma unroll
     for (int d = 0; d < NB; ++d)
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
             float o[4];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) o[x] = lse2 == INFINITY ? 0.f : acc[d][e + x] * a.scale;      // saw nothing: zeros
+            for (int x = 0; x < 4; ++x) o[x] = lse2 == INFINITY ? 0.f : acc[d][e + x] * back;      // saw nothing: zeros
             store4<T>(out, d * 32 + reg_row(e), a.D, a.out_vec, o);
         }
 }
@@ -704,7 +730,7 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_kernel(const AttnArgs a)
 // ---- dk and dv -----------------------------------------------------------------------------------------------------------
 template <typename T, int DP, int NW, bool VEC>
 __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 2 && VEC && NW == 4 ? 2 : 1) void attention_dkv_kernel(const AttnArgs a) {
-    constexpr bool BOTH = sizeof(T) == 2 && DP <= 64;             // dS in two parts, see above
+    constexpr bool BOTH = sizeof(T) == 2 && DP <= 64, F16 = Mma<T>::F16;      // dS in two parts, see above; Range
     constexpr bool VLDS = DP == 128 && sizeof(T) == 2;
     constexpr int RT = VLDS ? 32 : tile_rows<T, DP>();
     constexpr int NT = NW * 64, BN = NW * 32, CK = Mma<T>::CK, E = Mma<T>::E, NC = DP / CK, NB = DP / 32, RB = RT / 32;
@@ -743,6 +769,8 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 2 && VEC && NW =
             if constexpr (!VLDS) vf[c] = fetch<T, VEC>(vr, c * CK + half * E, a.D, has);
         }
     }
+    Range range;                                                  // of the lane's key
+    float factor = 1.f;
     rs_f32x16 dk[NB], dv[NB];
 #pragma unroll
     for (int n = 0; n < NB; ++n)
@@ -796,7 +824,7 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 2 && VEC && NW =
         // a row that sees nothing, or is none: exp2(z - inf) = 0
         asm volatile("" : "+v"(r_lse), "+v"(r_delta));            // all lanes wait for them here (see settle)
         if (threadIdx.x < RT) {
-            s_lse[buf][threadIdx.x] = r0 + (int)threadIdx.x >= stop ? INFINITY : back_lse(r_lse);
+            s_lse[buf][threadIdx.x] = r0 + (int)threadIdx.x >= stop ? INFINITY : back_lse(r_lse) - P_SHIFT<T>;
             s_delta[buf][threadIdx.x] = r_delta;
         }
         feed_sync<VEC>();
@@ -831,6 +859,18 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 2 && VEC && NW =
                 for (int e = 0; e < 16; ++e)
                     if (n * 32 + reg_row(e) < hide) s[e] = dp[e] = 0.f;
             }
+            if constexpr (F16) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) dp[e] *= factor;
+                const float top = half_max(reg_max(dp));
+                if (__any(range.past(top))) {
+                    const int by = range.follow(top);
+                    factor = ldexpf(factor, by);
+                    scale_by(dp, by);
+#pragma unroll
+                    for (int d = 0; d < NB; ++d) scale_by(dk[d], by);
+                }
+            }
 #pragma unroll
             for (int c = 0; c < 32 / CK; ++c) {
                 const V p = pack<T>(s, c), ds = pack<T>(dp, c);
@@ -846,6 +886,7 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 2 && VEC && NW =
     }
     if (key >= a.Tk) return;
     const long long at = (((long long)b * a.Tk + key) * a.Hk + hk) * a.D;
+    const float back = a.scale * P_UNIT<T> * range.unit();
 #pragma unroll
     for (int d = 0; d < NB; ++d)
 #pragma unroll
@@ -853,8 +894,8 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 2 && VEC && NW =
             float o[4], u[4];
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-                o[x] = has ? dk[d][e + x] * a.scale : 0.f;
-                u[x] = has ? dv[d][e + x] : 0.f;
+                o[x] = has ? dk[d][e + x] * back : 0.f;
+                u[x] = has ? dv[d][e + x] * P_UNIT<T> : 0.f;
             }
             if (a.splits > 1) {
                 const long long total = (long long)a.B * a.Tk * a.Hk * a.D;

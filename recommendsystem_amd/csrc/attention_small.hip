@@ -173,7 +173,7 @@ __global__ __launch_bounds__(64) void attention_small_fwd_kernel(const AttnArgs 
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                s[n][e] = __builtin_amdgcn_exp2f(s[n][e] * scale2 - base);
+                s[n][e] = __builtin_amdgcn_exp2f(s[n][e] * scale2 - (base - P_SHIFT<T>));
                 l += s[n][e];
             }
         l = col_sum(l);
@@ -189,7 +189,7 @@ __global__ __launch_bounds__(64) void attention_small_fwd_kernel(const AttnArgs 
         if (i >= a.Tq) continue;
         const bool none = l == 0.f;                               // nothing seen: zeros, whatever the other rows' keys hold
         const float inv = 1.f / l;
-        if (a.lse && g == 0) a.lse[((long long)b * Hq + h) * a.Tq + i] = none ? -INFINITY : (m + log2f(l)) * LN2;
+        if (a.lse && g == 0) a.lse[((long long)b * Hq + h) * a.Tq + i] = none ? -INFINITY : (m + log2f(l) - P_SHIFT<T>) * LN2;
         T* out = (T*)a.out + (((long long)b * a.Tq + i) * Hq + h) * a.D;
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
@@ -206,6 +206,7 @@ __global__ __launch_bounds__(64) void attention_small_fwd_kernel(const AttnArgs 
 template <typename T, int DP, int NT, bool VEC>
 __global__ __launch_bounds__(64) void attention_small_bwd_kernel(const AttnArgs a) {
     constexpr int CK = Mma16<T>::CK, TILES = Mma16<T>::TILES, NC = DP / CK, ND = DP / 16, R = 16 * TILES;
+    constexpr bool F16 = P_SHIFT<T> != 0.f;
     typedef typename Mma16<T>::V V;
     typedef Rows<T, DP> L;
     typedef Rows<T, NT * 16> LP;
@@ -230,6 +231,7 @@ __global__ __launch_bounds__(64) void attention_small_bwd_kernel(const AttnArgs 
     for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int d = 0; d < ND; ++d) dk[n][d] = dv[n][d] = rs_f32x4{0.f, 0.f, 0.f, 0.f};
+    Range range;                                                  // of all rows and keys: dS of a turn goes into one product
     // a turn is R rows of one head; loads run one turn ahead, as does the lanes' lse
     float lse[TILES];
     const int per_head = (a.Tq + R - 1) / R, turns = per_head * a.G;
@@ -254,13 +256,15 @@ __global__ __launch_bounds__(64) void attention_small_bwd_kernel(const AttnArgs 
         wave_sync();
         float lse2[TILES];
 #pragma unroll
-        for (int t = 0; t < TILES; ++t) lse2[t] = back_lse(lse[t]);
+        for (int t = 0; t < TILES; ++t) lse2[t] = back_lse(lse[t]) - P_SHIFT<T>;
         if (turn + 1 < turns) load(turn + 1);
+        rs_f32x4 all[TILES][NT];
+        float most = 0.f;
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
             const int i = i0 + t * 16 + col, lim = limit(a, part, i);
-            rs_f32x4 p[NT], ds[NT];
-            float delta = 0.f;
+            rs_f32x4 p[NT], (&ds)[NT] = all[t];
+            float delta = 0.f, top = 0.f;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 p[n] = ds[n] = rs_f32x4{0.f, 0.f, 0.f, 0.f};
@@ -277,21 +281,37 @@ __global__ __launch_bounds__(64) void attention_small_bwd_kernel(const AttnArgs 
                     delta += p[n][e] * ds[n][e];
                 }
             }
-            delta = col_sum(delta);
+            delta = col_sum(delta) * P_UNIT<T>;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) ds[n][e] = p[n][e] * (ds[n][e] - delta);
+                for (int e = 0; e < 4; ++e) {
+                    ds[n][e] = p[n][e] * (ds[n][e] - delta);
+                    top = fmaxf(top, fabsf(ds[n][e]));
+                }
                 // row = query: four consecutive keys of one row
                 store4<T>(s_p + (t * 16 + col) * LP::RS, n * 16 + 4 * g, NT * 16, true, (const float*)&p[n]);
-                store4<T>(s_d + (t * 16 + col) * LP::RS, n * 16 + 4 * g, NT * 16, true, (const float*)&ds[n]);
+                if constexpr (!F16) store4<T>(s_d + (t * 16 + col) * LP::RS, n * 16 + 4 * g, NT * 16, true, (const float*)&ds[n]);
+            }
+            float back = a.scale;                                 // dq takes a factor for each row
+            rs_f32x4 own[NT];
+            if constexpr (F16) {
+                top = col_max(top);
+                most = fmaxf(most, top);
+                Range row;
+                const int by = row.follow(top);
+                back *= P_UNIT<T> * row.unit();
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) own[n][e] = ldexpf(ds[n][e], by);
             }
             rs_f32x4 dq[ND];
 #pragma unroll
             for (int d = 0; d < ND; ++d) dq[d] = rs_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int n = 0; n < NT; n += TILES) {
-                const V x = pack<T>(ds + n);
+                const V x = pack<T>((F16 ? own : ds) + n);
 #pragma unroll
                 for (int d = 0; d < ND; ++d) dq[d] = Mma16<T>::mul(L::cols(s_k, n * 16, d * 16), x, dq[d]);
             }
@@ -301,10 +321,31 @@ __global__ __launch_bounds__(64) void attention_small_bwd_kernel(const AttnArgs 
                 for (int d = 0; d < ND; ++d) {
                     float x[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = lim == 0 || lse2[t] == INFINITY ? 0.f : dq[d][e] * a.scale;      // saw nothing
+                    for (int e = 0; e < 4; ++e) x[e] = lim == 0 || lse2[t] == INFINITY ? 0.f : dq[d][e] * back;      // saw nothing
                     store4<T>(out, d * 16 + 4 * g, a.D, a.out_vec, x);
                 }
             }
+        }
+        if constexpr (F16) {
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
+            const int by = range.follow(ldexpf(most, range.exp));
+            if (by != 0)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int d = 0; d < ND; ++d)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) dk[n][d][e] = ldexpf(dk[n][d][e], by);
+#pragma unroll
+            for (int t = 0; t < TILES; ++t)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float x[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = ldexpf(all[t][n][e], range.exp);
+                    store4<T>(s_d + (t * 16 + col) * LP::RS, n * 16 + 4 * g, NT * 16, true, x);
+                }
         }
         wave_sync();
 #pragma unroll
@@ -317,6 +358,7 @@ __global__ __launch_bounds__(64) void attention_small_bwd_kernel(const AttnArgs 
             }
         }
     }
+    const float back = a.scale * P_UNIT<T> * range.unit();
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         const int key = n * 16 + col;
@@ -324,9 +366,10 @@ __global__ __launch_bounds__(64) void attention_small_bwd_kernel(const AttnArgs 
         const long long at = (((long long)b * a.Tk + key) * a.Hk + hk) * a.D;
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
-            const float x[4] = {dk[n][d][0] * a.scale, dk[n][d][1] * a.scale, dk[n][d][2] * a.scale, dk[n][d][3] * a.scale};
+            const float x[4] = {dk[n][d][0] * back, dk[n][d][1] * back, dk[n][d][2] * back, dk[n][d][3] * back};
+            const float y[4] = {dv[n][d][0] * P_UNIT<T>, dv[n][d][1] * P_UNIT<T>, dv[n][d][2] * P_UNIT<T>, dv[n][d][3] * P_UNIT<T>};
             store4<T>((T*)a.dk + at, d * 16 + 4 * g, a.D, a.out_vec, x);
-            store4<T>((T*)a.dv + at, d * 16 + 4 * g, a.D, a.out_vec, (const float*)&dv[n][d]);
+            store4<T>((T*)a.dv + at, d * 16 + 4 * g, a.D, a.out_vec, y);
         }
     }
 }

@@ -3,7 +3,7 @@ too, unless a test says otherwise."""
 import pytest
 import torch
 
-from test_attention_gpu import compare, inside, make, reference
+from test_attention_gpu import compare, half_step, inside, make, reference
 
 pytestmark = pytest.mark.gpu
 
@@ -73,3 +73,76 @@ def test_rows_that_see_nothing_stay_zero_beside_rows_of_infinite_keys(Tq, Tk, D,
                 dq = ops.attention_bwd(do, q, *kv, o, lse, **how)[0]
                 assert torch.equal(lse == -torch.inf, out.view(2, 1, Tq).expand_as(lse))
                 assert torch.count_nonzero(o[out]).item() == 0 and torch.count_nonzero(dq[out]).item() == 0, (name, fill, how)
+
+
+# fp16 gradients.  dS is rounded once and averages over the terms it is summed with like the result's own rounding, P as well
+# (dv), and so does o's in delta: sqrt(1 + 1 + 0.6) = 1.6 times the root mean square of one final rounding, whatever the size
+# of the gradients.  Held to twice that rounding.  (With dS and P as they are, fp16 loses their last bits below 2^-14.)
+def rounding(ref):
+    return (ref.half().double() - ref).square().sum(-1).sqrt()
+
+
+def off(got, ref):
+    return (got.double() - ref).square().sum(-1).sqrt()
+
+
+def gradients(q, k, v, do, **how):
+    from recommendsystem_amd import ops
+    o, lse = ops.attention_fwd(q, k, v, **how)
+    ref = reference(q, k, v, do, **how)
+    return [(n, g, ref[n][0]) for n, g in zip(("dq", "dk", "dv"), ops.attention_bwd(do, q, k, v, o, lse, **how))]
+
+
+@pytest.mark.parametrize("size", [1e-1, 1e-3, 1e-4, 1e-5])
+@pytest.mark.parametrize("B,T,Hq,Hk,D", [(1, 2048, 2, 1, 128), (1, 2048, 2, 1, 64), (3, 200, 4, 4, 32), (5, 60, 2, 1, 64), (6, 31, 2, 2, 128)])
+def test_fp16_gradients_of_any_size(B, T, Hq, Hk, D, size):
+    q, k, v, do = make(B, T, T, Hq, Hk, D, "f16", seed=T + D)
+    for name, got, ref in gradients(q, k, v, (do * size).half()):
+        assert off(got, ref).square().sum() <= 4 * rounding(ref).square().sum(), name
+
+
+@pytest.mark.parametrize("B,T,D", [(1, 700, 128), (1, 700, 64), (4, 60, 64)])
+def test_fp16_gradients_of_every_row_where_rows_differ(B, T, D):
+    """Rows whose gradients lie a factor of 10^4 apart: each row of dq by itself (64 or 128 elements of a row: up to three times
+    its rounding), dk and dv as a whole."""
+    q, k, v, do = make(B, T, T, 2, 1, D, "f16", seed=61)
+    do = (do * 10.0 ** -(torch.arange(T, device="cuda") * 7 % 5).view(1, -1, 1, 1)).half()
+    for name, got, ref in gradients(q, k, v, do):
+        if name == "dq":
+            assert bool((off(got, ref) <= 3 * rounding(ref)).all()), (off(got, ref) / rounding(ref)).max()
+        assert off(got, ref).square().sum() <= 4 * rounding(ref).square().sum(), name
+
+
+@pytest.mark.parametrize("B,T,D", [(2, 300, 128), (2, 300, 64), (3, 60, 64), (3, 30, 128)])
+def test_fp16_gradients_whose_terms_pass_the_type(B, T, D):
+    """dS beyond 65504 whose sums with small keys and queries are ordinary numbers."""
+    q, k, v, do = make(B, T, T, 2, 1, D, "f16", seed=62)
+    q, k, v, do = (q / 1024).half(), (k / 1024).half(), (v * 4096).half(), (do * 4096).half()
+    ds = (do.double().amax() * v.double().amax() / T * D ** 0.5)
+    assert ds > 65504
+    for name, got, ref in gradients(q, k, v, do):
+        assert bool(ref.abs().amax() < 65504)
+        assert off(got, ref).square().sum() <= 4 * rounding(ref).square().sum(), name
+
+
+@pytest.mark.parametrize("Tq,Tk,D", [(40, 3000, 64), (1, 5000, 128), (40, 60, 64), (130, 2000, 32)])
+def test_fp16_small_probabilities_keep_their_bits(Tq, Tk, D):
+    """One key takes nearly all and holds nothing, the others have 2^-20 each and all the value: o is their sum, off by a half
+    step for theirs and one for its own."""
+    from recommendsystem_amd import ops
+    q, k = (torch.zeros(2, t, 1, D, device="cuda").half() for t in (Tq, Tk))
+    q[..., 0] = 1
+    k[:, 7, 0, 0] = 14.2
+    v = torch.zeros(2, Tk, 1, D, device="cuda").half()
+    v[:] = (1000 * torch.rand(1, 1, 1, D, device="cuda") + 100).half()
+    v[:, 7] = 0
+    do = torch.full_like(q, 1024.0)
+    o, lse = ops.attention_fwd(q, k, v, scale=1.0)
+    ref = reference(q, k, v, do, scale=1.0)
+    inside(o, ref["o"][0], 2.1 * half_step(torch.float16, ref["o"][0]), "o")
+    inside(lse, *ref["lse"], "lse")
+    dv = ops.attention_bwd(do, q, k, v, o, lse, scale=1.0)[2]
+    # dv: the same two half steps; beyond 65520 (the one key's, over 1024 x 64 rows) the type's value is infinite
+    past = ref["dv"][0].abs() >= 65520
+    assert bool((dv[past] == torch.inf).all()) and bool(past.any()) == (Tq > 64)
+    inside(dv[~past], ref["dv"][0][~past], 2.1 * half_step(torch.float16, ref["dv"][0][~past]), "dv")

@@ -57,10 +57,10 @@ template <typename T, bool WHOLE> __device__ __forceinline__ void rs_store(T* p,
     }
 }
 
-// Any number of workgroups (a grid dimension holds 2^32 lanes): kernels launched so take rs_block_id() for their number
-// and leave when it is past the last one.
+// Any number of workgroups: kernels launched so take rs_block_id() for their number and leave when it is past the last one.
+// A grid dimension holds fewer than 2^32 lanes, which 2^21 workgroups of up to 1024 keep.
 static inline dim3 rs_grid(long long blocks) {
-    const long long x = blocks < (1 << 22) ? blocks : (1 << 22);
+    const long long x = blocks < (1 << 21) ? blocks : (1 << 21);
     return dim3((unsigned)x, (unsigned)((blocks + x - 1) / x));
 }
 __device__ __forceinline__ long long rs_block_id() { return (long long)blockIdx.y * gridDim.x + blockIdx.x; }

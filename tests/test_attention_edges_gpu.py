@@ -146,3 +146,94 @@ def test_fp16_small_probabilities_keep_their_bits(Tq, Tk, D):
     past = ref["dv"][0].abs() >= 65520
     assert bool((dv[past] == torch.inf).all()) and bool(past.any()) == (Tq > 64)
     inside(dv[~past], ref["dv"][0][~past], 2.1 * half_step(torch.float16, ref["dv"][0][~past]), "dv")
+
+
+def backward_floats(kind, q, k):
+    """The large kernels' backward keeps delta in a workspace, the ones for few keys need none."""
+    from recommendsystem_amd import _lib
+    (B, Tq, Hq, D), (Tk, Hk) = q.shape, k.shape[1:3]
+    return _lib.lib().rs_attention_bwd_workspace_floats(("f32", "bf16", "f16").index(kind), B, Tq, Tk, Hq, Hk, D, 0)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("T,D", [(150, 64), (150, 128), (45, 32)])
+def test_strides_and_orders_of_both_sizes(T, D, kind):
+    """The strides of a user's tensors, for the kernels that take tiles through buffer descriptors and those for few keys."""
+    B, H = 2, 6
+    g = torch.Generator(device="cuda").manual_seed(T + D)
+    rn = lambda *s: torch.randn(*s, device="cuda", generator=g).to(make(1, 1, 1, 1, 1, 1, kind, 0)[0].dtype)      # noqa: E731
+    qkv, do = rn(B, T, 3 * H, D), rn(B, T, H, D)
+    assert (backward_floats(kind, qkv[:, :, :H], qkv[:, :, H:2 * H]) > 0) == (T > 64)
+    compare(qkv[:, :, :H], qkv[:, :, H:2 * H], qkv[:, :, 2 * H:], do)
+    heads_first = qkv.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3)
+    compare(heads_first[:, :, :H], heads_first[:, :, H:H + 2], heads_first[:, :, -2:], do.permute(2, 0, 1, 3).contiguous().permute(1, 2, 0, 3))
+    n = D - 5
+    compare(qkv[..., 1:n + 1][:, :, :H], qkv[..., 2:n + 2][:, :, H:2 * H], qkv[..., 3:n + 3][:, :, 2 * H:], do[..., :n], causal=True)      # unaligned
+    n = D - 8
+    compare(qkv[..., 1:n + 1][:, :, :H], qkv[..., 2:n + 2][:, :, H:2 * H], qkv[..., 3:n + 3][:, :, 2 * H:], do[..., :n], causal=True)
+    dims = qkv.transpose(2, 3)                                                            # last dimension not contiguous
+    compare(dims[..., :8][:, :, :4], dims[..., 8:16][:, :, :2], dims[..., 2:10][:, :, :2], do.transpose(2, 3)[:, :, :4, :6].repeat(1, 1, 1, 2)[..., :8])
+    compare(qkv[:1, :, :H].expand(B, T, H, D), qkv[:, :1, :H].expand(B, T, H, D), qkv[:, :, :1].expand(B, T, H, D), do[:, :1].expand(B, T, H, D))
+    compare(qkv[:, :, :H], qkv[:1, :, :1].expand(B, T, H, D), qkv[:1, :, 1:2].expand(B, T, H, D), do[:, :, :1].expand(B, T, H, D))
+    compare(qkv.flip(1)[:, :, :H], qkv[:, ::3, H:2 * H], qkv[:, 1:T:3, 2 * H:][:, :T // 3 + T % 3], do)
+    wide = rn(B, T, 3 * H, 2 * D)                                                         # every second head, half of each, from a column on
+    compare(wide[:, :, 0:2 * H:2, :D], wide[:, :, 1:2 * H:2, D:], wide[:, :, 2 * H:, D // 2:D // 2 + D], do)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("Tq,D", [(1, 64), (3, 128), (40, 64)])
+def test_strides_of_a_cache(Tq, D, kind):
+    """Few rows over a long cache that lies inside a wider one, heads first, with an expanded key head, unaligned."""
+    B, Tk, H = 2, 3000, 2
+    q, k, v, _ = make(B, Tq, Tk, 2 * H, H, D, kind, seed=71)
+    wide = torch.randn(B, Tk + 100, 2 * H, D + 3, device="cuda").to(q.dtype)
+    compare(q, wide[:, 50:50 + Tk, :H, :D], wide[:, 50:50 + Tk, H:, 3:], None)
+    hf = lambda x: x.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3)                 # noqa: E731
+    compare(hf(q), hf(k), hf(v), None, causal=True)
+    compare(q, k[:, :, :1].expand(B, Tk, H, D), v[:1].expand(B, Tk, H, D), None)
+    compare(q[..., 1:D - 2], k[..., 1:D - 2], v[..., 3:], None)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("Tq,D", [(150, 64), (150, 128), (1, 64), (40, 64)])
+def test_far_offsets(Tq, D, kind):
+    """Samples 2^31 elements apart, and rows 2^22 and more apart (past what a descriptor's tile may span): keys of a cache whose
+    rows hold every layer."""
+    T, B, H = 150, 2, 2
+    far = (1 << 31) + 4096
+    dtype = make(1, 1, 1, 1, 1, 1, kind, 0)[0].dtype
+    store = torch.empty(far + T * 3 * H * D, device="cuda", dtype=dtype)
+    qkv = store.as_strided((B, T, 3 * H, D), (far, 3 * H * D, D, 1))
+    qkv.copy_(torch.randn(B, T, 3 * H, D, device="cuda"))
+    do = torch.randn(B, Tq, H, D, device="cuda").to(dtype)
+    assert backward_floats(kind, do, qkv[:, :, H:2 * H]) > 0
+    compare(qkv[:, :Tq, :H], qkv[:, :, H:2 * H], qkv[:, :, 2 * H:], do, causal=True)
+    del store, qkv
+    for apart in ((1 << 22) - 8, 1 << 22, (1 << 24) + 8):        # the widest rows of the asynchronous loads, and past them
+        store = torch.empty((T + 1) * apart, device="cuda", dtype=dtype)
+        rows = store.as_strided((1, T, 3 * H, D), (T * apart, apart, D, 1))
+        rows.copy_(torch.randn(1, T, 3 * H, D, device="cuda"))
+        compare(rows[:, :Tq, :H], rows[:, :, H:2 * H], rows[:, :, 2 * H:], do[:1])
+        del store, rows
+
+
+@pytest.mark.parametrize("kind,D", [("bf16", 100), ("f16", 100), ("f32", 127), ("bf16", 65), ("f32", 102), ("f16", 127)])
+@pytest.mark.parametrize("Tq,Tk", [(150, 150), (50, 150), (50, 50), (130, 64)])
+def test_backward_of_wide_heads_that_are_not_aligned(Tq, Tk, D, kind):
+    q, k, v, do = make(2, Tq, Tk, 4, 2, D, kind, seed=D + Tq)
+    compare(q, k, v, do)
+    compare(q, k, v, do, causal=True)
+    n = torch.tensor([Tk, Tk // 3], device="cuda", dtype=torch.int32)
+    compare(q, k, v, do, lengths=n, query_lengths=n.clamp(max=Tq), causal=True)
+
+
+@pytest.mark.parametrize("Tq,G,D", [(1, 4, 7), (1, 1, 63), (2, 8, 7), (5, 3, 63), (1, 2, 33), (3, 1, 101), (1, 16, 30)])
+def test_single_tokens_of_odd_heads_in_fp32(Tq, G, D):
+    B, Tk, Hk = 3, 1003, 2
+    q, k, v, _ = make(B, Tq, Tk, G * Hk, Hk, D, "f32", seed=D)
+    n = torch.tensor([1003, 0, 517], device="cuda", dtype=torch.int32)
+    compare(q, k, v, None)
+    compare(q, k, v, None, lengths=n)
+    compare(q, k, v, None, causal=True)
+    pad = lambda x: torch.nn.functional.pad(x, (1, 2))[..., 1:-2]       # noqa: E731  unaligned rows of an odd stride
+    compare(pad(q), pad(k), pad(v), None, lengths=n, causal=True, query_start=n - Tq)

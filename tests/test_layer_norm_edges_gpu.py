@@ -3,7 +3,7 @@ unless a test says otherwise."""
 import pytest
 import torch
 
-from test_layer_norm_gpu import U, inside
+from test_layer_norm_gpu import U, compare, inside, make
 
 pytestmark = pytest.mark.gpu
 
@@ -21,3 +21,15 @@ def test_more_parameter_sums_than_a_grid_dimension_holds():
     for part in (slice(0, 1000), slice(N // 2, N // 2 + 1000), slice(N - 1000, N)):
         ref = dy[0, part].double() * ((x[0, part].double() - mean.double()) * rstd.double())
         inside(dw[part], ref, 4 * U * ref.abs(), "dw")
+
+
+@pytest.mark.parametrize("kind,wkind", [("f32", "f32"), ("bf16", "f32"), ("f16", "f16")])
+@pytest.mark.parametrize("M,N", [(2100, 5000), (1100, 16400), (2100, 4097), (1030, 16384), (3000, 1100)])
+def test_workgroups_of_wide_rows_meet_several(M, N, kind, wkind):
+    """More rows than the backward has workgroups: of one wide row each, and of a row longer than the registers hold."""
+    compare(*make(M, N, kind, wkind, residual=N % 2 == 0, seed=M + N))
+
+
+def test_wide_rows_at_odd_addresses():
+    x, r, w, b, dy, ds = make(1500, 5003, "bf16", "f32", True, seed=77)
+    compare(x[:, 2:], r[:, 1:-1], w[2:], b[2:].clone(), dy[:, :-2], ds[:, 2:])

@@ -237,3 +237,12 @@ def test_single_tokens_of_odd_heads_in_fp32(Tq, G, D):
     compare(q, k, v, None, causal=True)
     pad = lambda x: torch.nn.functional.pad(x, (1, 2))[..., 1:-2]       # noqa: E731  unaligned rows of an odd stride
     compare(pad(q), pad(k), pad(v), None, lengths=n, causal=True, query_start=n - Tq)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("Tq,Tk,D", [(899, 899, 64), (900, 900, 64), (70, 901, 40), (130, 1023, 64), (200, 895, 64)])
+def test_key_tiles_of_both_sizes(Tq, Tk, D, kind):
+    q, k, v, do = make(2, Tq, Tk, 3, 1, D, kind, seed=Tq + Tk)
+    compare(q, k, v, do)
+    n = torch.tensor([Tk - 3, Tk // 2], device="cuda", dtype=torch.int32)
+    compare(q, k, v, do, causal=True, lengths=n, query_lengths=n.clamp(max=Tq))

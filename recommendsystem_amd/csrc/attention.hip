@@ -947,38 +947,27 @@ int splits_for(int dtype, int B, int Tq, int Tk, int Hk, int G, int D) {
 
 // Shares of the rows for dk and dv.  Even work: split until there are two workgroups for every CU.  A causal mask or lengths
 // give the key tiles uneven work, and one workgroup per key tile leaves some CUs with twice the mean: split until there are
-// four (causal or ragged, dk / dv with their join at two and at four workgroups: 2 x 8192 x 4 key heads of 128 1847, 1161 us; 16384
-// x 2 of 128 1803, 1730; 2 x 4096 x 8 of 128 200, 147; 2 x 2048 x 4 of 128 143, 128; 4 x 2048 x 8 of 64 75, 70; of 32 51, 48;
-// the join costs more than it gives for the shortest: 16 x 1000 x 4 of 64 39, 45, 4096 x 2 of 64 93, 102.  Without a mask as
-// many tiles as the first takes 1.20 ms in one share, 1.34 in four).  No share is shorter than eight row tiles.
+// four (2 x 8192 causal, 4 key heads, 512 key tiles: 1.79 ms in one share, 1.34 in two; without the mask one share
+// of as many tiles takes 1.20 ms, four 1.34).  No share is shorter than eight row tiles.
 int dkv_splits(int B, int Tq, int Tk, int Hk, int G, int uneven) {
     const long long units = (long long)B * Hk * rs_cdiv(Tk, Tk <= 64 ? 64 : 128), turns = (long long)G * rs_cdiv(Tq, 64);
     const long long want = (uneven ? 1024 : 512) / units, most = turns / 8, s = want < most ? want : most;
     return s < 1 ? 1 : s > 16 ? 16 : (int)s;
 }
 
-// KT: keys at a time.
-template <typename T, int DP, int NW, int KT> void launch_fwd_tiles(const AttnArgs& a, dim3 grid, hipStream_t stream) {
-    if (a.vec) hipLaunchKernelGGL((attention_fwd_kernel<T, DP, NW, KT, true>), grid, dim3(NW * 64), 0, stream, a);
-    else hipLaunchKernelGGL((attention_fwd_kernel<T, DP, NW, KT, false>), grid, dim3(NW * 64), 0, stream, a);
-}
 template <typename T, int DP, int NW> int launch_fwd(AttnArgs a, hipStream_t stream) {
+    // heads of 64: more keys at a time give the wave four independent chains of products (1537 x 12 heads x 3 fp16: 64 keys
+    // 50.5 us, 128 45.1); heads of 128 have no registers for it
+    constexpr int KT = NW == 1 ? 32 : NW == 4 && DP == 64 && sizeof(T) == 2 ? 128 : tile_rows<T, DP>();
     const dim3 grid = rs_grid(order_units(a));
-    // Heads of 33..64 in 16 bits over long keys: 128 at a time give the wave four independent chains of products; heads of 128
-    // have no registers for it, short samples too few tiles (1537 keys x 12 heads x 3 fp16: 64 at a time 47.6 us, 128 42.1; 1000
-    // keys 34.8, 30.6; 800, causal, 35.6, 37.8; 600 30.1, 30.4; 400 52.0, 60.7; ragged histories of up to 200 50, 64 and of up
-    // to 70 19.7, 26.7)
-    constexpr bool WIDE = NW == 4 && DP == 64 && sizeof(T) == 2;
+    const bool few = NW == 1 && sizeof(T) == 4 && a.Tq * a.G <= 16;
     if constexpr (NW == 1 && sizeof(T) == 4) {
         constexpr int FEW = DP == 128 ? 16 : 32;
-        if (a.Tq * a.G > 16) launch_fwd_tiles<T, DP, NW, 32>(a, grid, stream);
-        else if (a.vec) hipLaunchKernelGGL((attention_few_fwd_kernel<DP, FEW, true>), grid, dim3(64), 0, stream, a);
-        else hipLaunchKernelGGL((attention_few_fwd_kernel<DP, FEW, false>), grid, dim3(64), 0, stream, a);
-    } else if (WIDE && a.Tk >= 900) {
-        launch_fwd_tiles<T, DP, NW, WIDE ? 128 : tile_rows<T, DP>()>(a, grid, stream);
-    } else {
-        launch_fwd_tiles<T, DP, NW, NW == 1 ? 32 : tile_rows<T, DP>()>(a, grid, stream);
+        if (few && a.vec) hipLaunchKernelGGL((attention_few_fwd_kernel<DP, FEW, true>), grid, dim3(64), 0, stream, a);
+        else if (few) hipLaunchKernelGGL((attention_few_fwd_kernel<DP, FEW, false>), grid, dim3(64), 0, stream, a);
     }
+    if (!few && a.vec) hipLaunchKernelGGL((attention_fwd_kernel<T, DP, NW, KT, true>), grid, dim3(NW * 64), 0, stream, a);
+    else if (!few) hipLaunchKernelGGL((attention_fwd_kernel<T, DP, NW, KT, false>), grid, dim3(NW * 64), 0, stream, a);
     RS_CHECK_LAUNCH("rs_attention_fwd");
     if (a.splits > 1) {
         hipLaunchKernelGGL((attention_join_kernel<T>), rs_grid(((long long)a.B * a.Hk * a.Tq * a.G + 7) / 8), dim3(256), 0, stream, a);

@@ -955,19 +955,28 @@ int dkv_splits(int B, int Tq, int Tk, int Hk, int G, int uneven) {
     return s < 1 ? 1 : s > 16 ? 16 : (int)s;
 }
 
+// KT: keys at a time.
+template <typename T, int DP, int NW, int KT> void launch_fwd_tiles(const AttnArgs& a, dim3 grid, hipStream_t stream) {
+    if (a.vec) hipLaunchKernelGGL((attention_fwd_kernel<T, DP, NW, KT, true>), grid, dim3(NW * 64), 0, stream, a);
+    else hipLaunchKernelGGL((attention_fwd_kernel<T, DP, NW, KT, false>), grid, dim3(NW * 64), 0, stream, a);
+}
 template <typename T, int DP, int NW> int launch_fwd(AttnArgs a, hipStream_t stream) {
-    // heads of 64: more keys at a time give the wave four independent chains of products (1537 x 12 heads x 3 fp16: 64 keys
-    // 50.5 us, 128 45.1); heads of 128 have no registers for it
-    constexpr int KT = NW == 1 ? 32 : NW == 4 && DP == 64 && sizeof(T) == 2 ? 128 : tile_rows<T, DP>();
     const dim3 grid = rs_grid(order_units(a));
-    const bool few = NW == 1 && sizeof(T) == 4 && a.Tq * a.G <= 16;
+    // Heads of 33..64 in 16 bits over long keys: 128 at a time give the wave four independent chains of products; heads of 128
+    // have no registers for it, short samples too few tiles (1537 keys x 12 heads x 3 fp16: 64 at a time 47.6 us, 128 42.1; 1000
+    // keys 34.8, 30.6; 800, causal, 35.6, 37.8; 600 30.1, 30.4; 400 52.0, 60.7; ragged histories of up to 200 50, 64 and of up
+    // to 70 19.7, 26.7)
+    constexpr bool WIDE = NW == 4 && DP == 64 && sizeof(T) == 2;
     if constexpr (NW == 1 && sizeof(T) == 4) {
         constexpr int FEW = DP == 128 ? 16 : 32;
-        if (few && a.vec) hipLaunchKernelGGL((attention_few_fwd_kernel<DP, FEW, true>), grid, dim3(64), 0, stream, a);
-        else if (few) hipLaunchKernelGGL((attention_few_fwd_kernel<DP, FEW, false>), grid, dim3(64), 0, stream, a);
+        if (a.Tq * a.G > 16) launch_fwd_tiles<T, DP, NW, 32>(a, grid, stream);
+        else if (a.vec) hipLaunchKernelGGL((attention_few_fwd_kernel<DP, FEW, true>), grid, dim3(64), 0, stream, a);
+        else hipLaunchKernelGGL((attention_few_fwd_kernel<DP, FEW, false>), grid, dim3(64), 0, stream, a);
+    } else if (WIDE && a.Tk >= 900) {
+        launch_fwd_tiles<T, DP, NW, WIDE ? 128 : tile_rows<T, DP>()>(a, grid, stream);
+    } else {
+        launch_fwd_tiles<T, DP, NW, NW == 1 ? 32 : tile_rows<T, DP>()>(a, grid, stream);
     }
-    if (!few && a.vec) hipLaunchKernelGGL((attention_fwd_kernel<T, DP, NW, KT, true>), grid, dim3(NW * 64), 0, stream, a);
-    else if (!few) hipLaunchKernelGGL((attention_fwd_kernel<T, DP, NW, KT, false>), grid, dim3(NW * 64), 0, stream, a);
     RS_CHECK_LAUNCH("rs_attention_fwd");
     if (a.splits > 1) {
         hipLaunchKernelGGL((attention_join_kernel<T>), rs_grid(((long long)a.B * a.Hk * a.Tq * a.G + 7) / 8), dim3(256), 0, stream, a);

@@ -947,8 +947,10 @@ int splits_for(int dtype, int B, int Tq, int Tk, int Hk, int G, int D) {
 
 // Shares of the rows for dk and dv.  Even work: split until there are two workgroups for every CU.  A causal mask or lengths
 // give the key tiles uneven work, and one workgroup per key tile leaves some CUs with twice the mean: split until there are
-// four (2 x 8192 causal, 4 key heads, 512 key tiles: 1.79 ms in one share, 1.34 in two; without the mask one share
-// of as many tiles takes 1.20 ms, four 1.34).  No share is shorter than eight row tiles.
+// four (causal or ragged, dk / dv with their join at two and at four workgroups: 2 x 8192 x 4 key heads of 128 1847, 1161 us; 16384
+// x 2 of 128 1803, 1730; 2 x 4096 x 8 of 128 200, 147; 2 x 2048 x 4 of 128 143, 128; 4 x 2048 x 8 of 64 75, 70; of 32 51, 48;
+// the join costs more than it gives for the shortest: 16 x 1000 x 4 of 64 39, 45, 4096 x 2 of 64 93, 102.  Without a mask as
+// many tiles as the first takes 1.20 ms in one share, 1.34 in four).  No share is shorter than eight row tiles.
 int dkv_splits(int B, int Tq, int Tk, int Hk, int G, int uneven) {
     const long long units = (long long)B * Hk * rs_cdiv(Tk, Tk <= 64 ? 64 : 128), turns = (long long)G * rs_cdiv(Tq, 64);
     const long long want = (uneven ? 1024 : 512) / units, most = turns / 8, s = want < most ? want : most;

@@ -2042,6 +2042,8 @@ def attention_bwd(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.T
     """Gradients (dq, dk, dv) of attention_fwd's o from do, with the same arguments and the forward's o and lse; the
     probabilities are computed again.  Shared key heads get the sum over their query heads.  No atomics: the same bits
     every time."""
+    if o is None or lse is None:
+        raise RSError("attention_bwd: needs the forward's o and lse (want_lse=True)")
     code, q, k, v, (B, Tq, Tk, Hq, Hk, D), how, _ = _attention_args(q, k, v, lengths, query_lengths, causal, query_start, scale)
     do = _heads_view(do, "do", q.shape, q.dtype)
     o = _heads_view(o, "o", q.shape, q.dtype)

@@ -3,7 +3,7 @@ too, unless a test says otherwise."""
 import pytest
 import torch
 
-from test_attention_gpu import compare, half_step, inside, make, reference
+from test_attention_gpu import U, compare, half_step, inside, make, reference
 
 pytestmark = pytest.mark.gpu
 
@@ -246,3 +246,19 @@ def test_key_tiles_of_both_sizes(Tq, Tk, D, kind):
     compare(q, k, v, do)
     n = torch.tensor([Tk - 3, Tk // 2], device="cuda", dtype=torch.int32)
     compare(q, k, v, do, causal=True, lengths=n, query_lengths=n.clamp(max=Tq))
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("Tq,Tk,D", [(150, 150, 64), (40, 60, 32), (3, 2000, 128), (150, 1000, 64)])
+def test_scores_of_millions(Tq, Tk, D, kind):
+    """Scores whose last bits are worth tenths: which key a row takes is up to their rounding, but what it gets lies within the
+    values, and every gradient is finite."""
+    from recommendsystem_amd import ops
+    q, k, v, do = make(2, Tq, Tk, 4, 2, D, kind, seed=81)
+    q, k = q * 1000, k * 1000
+    o, lse = ops.attention_fwd(q, k, v)
+    assert bool((lse > 1e5).any()) and bool(torch.isfinite(lse).all())
+    hull = v.double().abs().amax(1).repeat_interleave(2, 1).unsqueeze(1)
+    assert bool((o.double().abs() <= hull * (1 + 2 * torch.finfo(v.dtype).eps + (Tk + 64) * U)).all())
+    for g in ops.attention_bwd(do, q, k, v, o, lse):
+        assert bool(torch.isfinite(g).all())

@@ -22,10 +22,11 @@
 // atomics, the same bits every time.  Query heads that share a key head lie next to one another as rows of the forward
 // and dq (row = position * group + head), so a cache is read once for all of them; dk / dv walk over them.
 //
-// Bound by the matrix cores for heads of 128 (2 x 8192 x 16 heads on 4 key heads, bf16, causal: forward 552 us = 1000 TFLOP/s,
-// dq 722 = 1140, dk / dv 1129 + 25 for the join = 950; a library product of 8192^3 reaches 1208 here), by the exponentials
+// Bound by the matrix cores for heads of 128 (2 x 8192 x 16 heads on 4 key heads, bf16, causal: forward 551 us = 1000 TFLOP/s,
+// dq 721 = 1140, dk / dv 1120 + 25 for the join = 960; a library product of 8192^3 reaches 1208 here), by the exponentials
 // and the latency of a wave's chain for smaller ones (1537 x 12 x 3 heads of 64, fp16: 41 us, 530 TFLOP/s), by memory for
-// single tokens over caches (1.07 GB of full caches in 188 us, 5.7 TB/s).
+// single tokens over caches (1.07 GB of full caches in 190 us, 5.6 TB/s).  Heads between the padded sizes of 32, 64 and 128 pay
+// for the padding: heads of 96 in the shape above 521, 667 and 1086 + 19 us.
 //
 // Roundings: products of 16-bit operands are exact and summed in fp32; P and dS are rounded to the operands' type for
 // their second product (the matrix cores take equal types; the rounding is a half step per element and averages out over
@@ -425,8 +426,8 @@ __global__ __launch_bounds__(NW * 64) void attention_fwd_kernel(const AttnArgs a
 }
 
 // At most 16 rows (single tokens, short chunks) in fp32, whose matrix instructions are slow enough to matter here: 16x16 tiles
-// do half the work of 32x32 ones padded from 16 columns (531 samples x 4 rows x 2 heads of 96 over caches of up to 7632:
-// 1155 -> 509 us, 3.0 TB/s; 64 tokens x 8 heads of 128 over 4096 keys each 390 us, 5.5 TB/s).  One wave, 16 or 32 keys at
+// do half the work of 32x32 ones padded from 16 columns (531 samples x 4 rows x 2 heads of 96 on one key head over caches of up
+// to 7632: 1155 -> 481 us, 3.2 TB/s; 64 tokens x 8 heads of 128 over 4096 keys each 385..420 us, 5.1 TB/s and up).  One wave, 16 or 32 keys at
 // a time; as above otherwise.
 template <int DP, int KT, bool VEC>
 __global__ __launch_bounds__(64) void attention_few_fwd_kernel(const AttnArgs a) {

@@ -11,7 +11,7 @@
 // over the rows, P and dS of a row tile go through a small LDS tile to be read the other way.  The query heads that
 // share a key head pass by one after the other, so every gradient has one owner.  A wave has a row's whole P and do . v, so
 // delta_i = sum_j p_ij (do_i . v_j), which is the same as do_i . o_i without o and its rounding.
-// 39 fields x 4096 samples, 2 heads of 16, fp32: forward 27 us (82 MB, 3.0 TB/s), backward 52 us (143 MB, 2.7 TB/s), of which
+// 39 fields x 4096 samples, 2 heads of 16, fp32: forward 27 us (82 MB, 3.0 TB/s), backward 53 us (143 MB, 2.7 TB/s), of which
 // 8 and 19 us are matrix instructions; what is left is the latency of each wave's one short chain.
 #include "attention.h"
 
@@ -423,8 +423,8 @@ int launch_any(int dtype, const AttnArgs& a, bool back, hipStream_t stream) {
 
 }  // namespace
 
-// Against the kernels of attention.hip, forward and backward: 512 x 60 x 8 heads of 64 bf16 29 + 70 us (30 + 90), 1024 x 30 x 8
-// of 128 bf16 61 + 132 (63 + 259), of 64 fp32 60 + 129 (71 + 469), 1024 x 16 x 8 of 128 fp32 59 + 112 (172 + 517).  Larger
+// Against the kernels of attention.hip, forward and backward: 512 x 60 x 8 heads of 64 bf16 29 + 71 us (30 + 90), 1024 x 30 x 8
+// of 128 bf16 61 + 120 (63 + 259), of 64 fp32 62 + 122 (71 + 469), 1024 x 16 x 8 of 128 fp32 60 + 104 (172 + 517).  Larger
 // products than these do not fit a wave's registers.
 bool rs_attention_small_ok(int dtype, int Tq, int Tk, int D) {
     const int most = dtype == RS_F32 ? (D <= 32 ? 64 : D <= 64 ? 32 : 16) : (D <= 64 ? 64 : 32);

@@ -13,8 +13,10 @@
 // The backward's workgroups walk over the rows in steps of the grid, so a lane meets the same columns in every row and
 // keeps their dw / db sums in registers; a workgroup adds up its row groups in LDS and writes one partial row, and a
 // second launch adds the partial rows in a fixed order (no atomics: the same bits every time).
-// 32768 x 4096 bf16 with a residual: forward 203 us (1.07 GB, 5.3 TB/s), backward 235 + 7 us (1.07 GB, 4.4 TB/s); a copy of
-// 4 GiB reaches 4.8.  4096 x 1024 fp32: 8.7 and 12.6 + 4.3 us.
+// 32768 x 4096 bf16 with a residual: forward 203 us (1.07 GB, 5.3 TB/s), backward 237 + 7 us (1.07 GB, 4.4 TB/s); a copy of
+// 4 GiB reaches 4.8.  4096 x 1024 fp32: 8.8 and 12.8 + 4.0 us: there each of 1024 workgroups has one row group, so the partial
+// rows (8.4 MB, 8 bytes for every element of up to 1024 row groups) are written for nothing that registers added up.
+// Rows beyond the registers: 2000 x 20001 bf16 107 us forward (160 MB, 1.5 TB/s), 210 + 43 backward (element by element).
 #include "lowp.h"
 #include "../../include/rs_hip.h"
 

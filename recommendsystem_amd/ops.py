@@ -2017,7 +2017,8 @@ def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: Op
     Row i of sample b sees key j where j < lengths[b] and i < query_lengths[b] (int32 [B], None: all) and, causal,
     j <= i + query_start: an int, an int32 [B], or None for Tk - Tq, which lines up the last row with the last key.  Rows
     that see nothing get zeros (lse -inf), and what lies behind the lengths is never used, whatever it holds.  A row whose scores
-    all overflow to -inf (float32 operands near 1e20) counts as one that sees nothing.
+    all overflow to -inf (float32 operands near 1e20) counts as one that sees nothing.  Within the lengths keys, values and
+    queries have to be finite: causal, a non-finite one may reach earlier rows, too.
     scale: D ** -0.5 by default, positive.  Returns (o, lse): o [B, Tq, Hq, D], lse [B, Hq, Tq] float32 or None."""
     code, q, k, v, (B, Tq, Tk, Hq, Hk, D), how, dev = _attention_args(q, k, v, lengths, query_lengths, causal, query_start, scale)
     o = torch.empty((B, Tq, Hq, D), dtype=q.dtype, device=dev)
